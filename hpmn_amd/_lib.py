@@ -10,7 +10,7 @@ import os
 from typing import Optional
 
 HPMN_MAX_LAYERS = 12
-HPMN_ABI_VERSION = 14
+HPMN_ABI_VERSION = 15
 HPMN_MAX_RANKS = 8
 HPMN_MAX_CHUNKS = 32
 HPMN_FWD_NO_CANDIDATE = 1
@@ -207,7 +207,41 @@ class HpmnTileFwd(C.Structure):
                 ("bc", C.c_void_p), ("y", C.c_void_p), ("h_last", C.c_void_p), ("h_last_stride", C.c_int64)]
 
 
+HPMN_F32, HPMN_BF16, HPMN_F16 = 0, 1, 2
+HPMN_GATED_SCAN_TILE = 128
+HPMN_STEP_COMMIT = 1
+HPMN_STEP_USER_I64 = 2
+HPMN_STEP_MAX_INDEXED = 4096
+
+
+class HpmnGatedScan(C.Structure):
+    _fields_ = [("B", C.c_int32), ("T", C.c_int32), ("C", C.c_int32), ("dtype", C.c_int32), ("period", C.c_int32), ("pad_", C.c_int32),
+                ("z", C.c_void_p), ("v", C.c_void_p), ("z_sb", C.c_int64), ("z_st", C.c_int64), ("v_sb", C.c_int64),
+                ("v_st", C.c_int64), ("begin", C.c_void_p), ("h0", C.c_void_p), ("h0_sb", C.c_int64), ("y", C.c_void_p),
+                ("y_sb", C.c_int64), ("y_st", C.c_int64), ("h_last", C.c_void_p), ("saved", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class HpmnGatedScanBwd(C.Structure):
+    _fields_ = [("B", C.c_int32), ("T", C.c_int32), ("C", C.c_int32), ("dtype", C.c_int32), ("period", C.c_int32), ("pad_", C.c_int32),
+                ("z", C.c_void_p), ("v", C.c_void_p), ("z_sb", C.c_int64), ("z_st", C.c_int64), ("v_sb", C.c_int64),
+                ("v_st", C.c_int64), ("begin", C.c_void_p), ("saved", C.c_void_p), ("d_y", C.c_void_p),
+                ("dy_sb", C.c_int64), ("dy_st", C.c_int64), ("d_h_last", C.c_void_p), ("d_z", C.c_void_p), ("d_v", C.c_void_p),
+                ("dz_sb", C.c_int64), ("dz_st", C.c_int64), ("dv_sb", C.c_int64), ("dv_st", C.c_int64), ("d_h0", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class HpmnGatedStep(C.Structure):
+    _fields_ = [("B", C.c_int32), ("C", C.c_int32), ("dtype", C.c_int32), ("flags", C.c_int32), ("z", C.c_void_p), ("v", C.c_void_p),
+                ("z_s", C.c_int64), ("v_s", C.c_int64), ("state", C.c_void_p), ("state_s", C.c_int64), ("n_users", C.c_int64),
+                ("user", C.c_void_p), ("y", C.c_void_p), ("y_s", C.c_int64)]
+
+
 SIGNATURES = {
+    "hpmn_gated_scan_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32]),
+    "hpmn_gated_scan_fwd": (C.c_int, [C.POINTER(HpmnGatedScan), C.c_void_p]),
+    "hpmn_gated_scan_bwd": (C.c_int, [C.POINTER(HpmnGatedScanBwd), C.c_void_p]),
+    "hpmn_gated_scan_step": (C.c_int, [C.POINTER(HpmnGatedStep), C.c_void_p]),
     "hpmn_abi_version": (C.c_int, []),
     "hpmn_strerror": (C.c_char_p, [C.c_int]),
     "hpmn_last_hip_error": (C.c_int, []),

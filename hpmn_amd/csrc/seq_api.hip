@@ -1,0 +1,77 @@
+// extern "C" entries of the sequence operators (include/hpmn_hip.h, ABI v15): argument validation and dispatch.
+#include "seq_types.h"
+
+namespace hpmn {
+
+size_t gated_scan_workspace_bytes(int B, int T, int C);
+int gated_scan_fwd_launch(const HpmnGatedScan &a, hipStream_t st);
+int gated_scan_bwd_launch(const HpmnGatedScanBwd &a, hipStream_t st);
+int gated_step_launch(const HpmnGatedStep &a, hipStream_t st);
+
+static inline bool known_dtype(int d) { return d == HPMN_F32 || d == HPMN_BF16 || d == HPMN_F16; }
+static inline bool aligned_to(const void *p, int dtype) { return is_aligned(p, elem_size(dtype)); }
+
+// One grid dimension and 32-bit block indices: (sequences) x (channel blocks) has to stay below 2^31.
+static inline bool scan_grid_ok(int B, int C) { return (long)B * ((C + 15) / 16) < (1l << 30); }
+
+}  // namespace hpmn
+
+using namespace hpmn;
+
+static inline void drop_stale_hip_error() { (void)hipGetLastError(); }
+
+extern "C" {
+
+size_t hpmn_gated_scan_workspace_bytes(int32_t B, int32_t T, int32_t C) {
+    if (B < 1 || T < 1 || C < 1 || !scan_grid_ok(B, C)) return 0;
+    return gated_scan_workspace_bytes(B, T, C);
+}
+
+int hpmn_gated_scan_fwd(const HpmnGatedScan *a, void *stream) {
+    drop_stale_hip_error();
+    if (!a) return HPMN_EINVAL;
+    if (a->B < 0 || a->T < 1 || a->C < 1 || a->period < 1 || a->T % a->period != 0 || !known_dtype(a->dtype)) return HPMN_EINVAL;
+    if (a->B == 0) return HPMN_OK;
+    if (!a->z || !a->v || !(a->y || a->h_last || a->saved)) return HPMN_EINVAL;
+    if (!aligned_to(a->z, a->dtype) || !aligned_to(a->v, a->dtype) || !aligned_to(a->y, a->dtype)) return HPMN_EINVAL;
+    if (a->z_sb < 0 || a->z_st < 0 || a->v_sb < 0 || a->v_st < 0 || a->h0_sb < 0 || a->y_sb < 0 || a->y_st < 0) return HPMN_EINVAL;
+    if (!scan_grid_ok(a->B, a->C)) return HPMN_EUNSUPPORTED;
+    const size_t need = gated_scan_workspace_bytes(a->B, a->T, a->C);
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need || !is_aligned(a->workspace, 16))) return HPMN_EINVAL;
+    return gated_scan_fwd_launch(*a, (hipStream_t)stream);
+}
+
+int hpmn_gated_scan_bwd(const HpmnGatedScanBwd *a, void *stream) {
+    drop_stale_hip_error();
+    if (!a) return HPMN_EINVAL;
+    if (a->B < 0 || a->T < 1 || a->C < 1 || a->period < 1 || a->T % a->period != 0 || !known_dtype(a->dtype)) return HPMN_EINVAL;
+    if (a->B == 0) return HPMN_OK;
+    if (!a->z || !a->v || !a->saved || !a->d_z || !a->d_v) return HPMN_EINVAL;
+    if (!aligned_to(a->z, a->dtype) || !aligned_to(a->v, a->dtype) || !aligned_to(a->d_y, a->dtype) || !aligned_to(a->d_z, a->dtype) ||
+        !aligned_to(a->d_v, a->dtype))
+        return HPMN_EINVAL;
+    if (a->z_sb < 0 || a->z_st < 0 || a->v_sb < 0 || a->v_st < 0 || a->dy_sb < 0 || a->dy_st < 0 || a->dz_sb < 0 || a->dz_st < 0 ||
+        a->dv_sb < 0 || a->dv_st < 0)
+        return HPMN_EINVAL;
+    if (!scan_grid_ok(a->B, a->C)) return HPMN_EUNSUPPORTED;
+    const size_t need = gated_scan_workspace_bytes(a->B, a->T, a->C);
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need || !is_aligned(a->workspace, 16))) return HPMN_EINVAL;
+    return gated_scan_bwd_launch(*a, (hipStream_t)stream);
+}
+
+int hpmn_gated_scan_step(const HpmnGatedStep *a, void *stream) {
+    drop_stale_hip_error();
+    if (!a) return HPMN_EINVAL;
+    if (a->B < 0 || a->C < 1 || a->n_users < 0 || !known_dtype(a->dtype)) return HPMN_EINVAL;
+    if (a->flags & ~(HPMN_STEP_COMMIT | HPMN_STEP_USER_I64)) return HPMN_EINVAL;
+    if (a->B == 0) return HPMN_OK;
+    if (!a->z || !a->v || (!a->state && a->n_users > 0) || !(a->y || (a->flags & HPMN_STEP_COMMIT))) return HPMN_EINVAL;
+    if (!a->user && a->B != a->n_users) return HPMN_EINVAL;
+    if (!aligned_to(a->z, a->dtype) || !aligned_to(a->v, a->dtype) || !aligned_to(a->y, a->dtype)) return HPMN_EINVAL;
+    if (a->z_s < 0 || a->v_s < 0 || a->y_s < 0 || a->state_s < a->C) return HPMN_EINVAL;
+    if (a->user && (a->flags & HPMN_STEP_COMMIT) && a->B > HPMN_STEP_MAX_INDEXED) return HPMN_EUNSUPPORTED;
+    if ((long)a->B * ((a->C + 3) / 4) >= (1l << 36)) return HPMN_EUNSUPPORTED;
+    return gated_step_launch(*a, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -1569,3 +1569,187 @@ def read_fwd_bwd_n(descs, params, d_params, memories, lasts, label, masks, keep_
                                           _ptr_array(d_mem), _ptr_array(d_last), d_params.data_ptr(), ws.data_ptr(), _stream())
     _lib.check(rc, "hpmn_read_fwd_bwd_n")
     return dict(prediction=pred, log_loss_sum=loss_out[0], memory_loss=loss_out[1], d_memory=d_mem, d_last=d_last)
+
+
+# ---------------------------------------------------------------------------------------
+# sequence operators: the gated linear recurrence (time-parallel counterpart of the GRU scans above)
+# ---------------------------------------------------------------------------------------
+_SEQ_DTYPES = {torch.float32: _lib.HPMN_F32, torch.bfloat16: _lib.HPMN_BF16, torch.float16: _lib.HPMN_F16}
+
+
+def _chk_seq(name, t, shape, dtype, device):
+    """A device tensor of the given shape / dtype whose last dimension is dense (the others may be strided)."""
+    if not (t.is_cuda and t.device == device and t.dtype == dtype and tuple(t.shape) == tuple(shape)):
+        raise ValueError("%s: expected %s %s on %s, got %s %s on %s" % (name, tuple(shape), dtype, device, tuple(t.shape), t.dtype, t.device))
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError("%s: the last dimension has to be dense, got strides %s" % (name, t.stride()))
+
+
+def _chk_out(name, t):
+    """An output's rows must not overlap: every stride in front of the dense last dimension covers a row."""
+    for d in range(t.dim() - 1):
+        if t.shape[d] > 1 and t.stride(d) < t.shape[-1]:
+            raise ValueError("%s: overlapping rows, strides %s" % (name, t.stride()))
+
+
+def _seq_input(name, t, ndim):
+    if t.dim() != ndim or not t.is_cuda or t.dtype not in _SEQ_DTYPES:
+        raise ValueError("%s: expected a %d-dimensional float32 / bfloat16 / float16 CUDA tensor, got %s %s on %s"
+                         % (name, ndim, tuple(t.shape), t.dtype, t.device))
+    return _SEQ_DTYPES[t.dtype]
+
+
+def _call_on(device, name, fn, a):
+    """fn(&a, stream) on the device's current stream, with that device current (a launch needs both to agree)."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(C.byref(a), torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(C.byref(a), torch.cuda.current_stream(device).cuda_stream)
+    _lib.check(rc, name)
+
+
+def _gated_scan_shape(z, v, begin, period):
+    _seq_input("z", z, 3)
+    B, T, Cc = z.shape
+    _chk_seq("z", z, (B, T, Cc), z.dtype, z.device)
+    _chk_seq("v", v, (B, T, Cc), z.dtype, z.device)
+    if begin is not None:
+        if not (begin.device == z.device and begin.dtype == torch.int32 and tuple(begin.shape) == (B,) and begin.is_contiguous()):
+            raise ValueError("begin: expected contiguous int32 [%d] on %s, got %s %s" % (B, z.device, begin.dtype, tuple(begin.shape)))
+    if period < 1 or T % period != 0:
+        raise ValueError("length %d not divisible by period %d" % (T, period))
+    return B, T, Cc
+
+
+def _gated_scan_workspace(B, T, Cc, device):
+    # per call: the caching allocator keeps it on the call's stream, and a captured graph owns its own
+    n = int(_lib.load().hpmn_gated_scan_workspace_bytes(B, T, Cc))
+    return (torch.empty(n, device=device, dtype=torch.uint8), n) if n else (None, 0)
+
+
+def gated_scan_fwd(z, v, *, h0=None, begin=None, period=1, train=False):
+    """hpmn_gated_scan_fwd: h_t = a_t h_{t-1} + (1 - a_t) v_t with a = sigmoid(z) over ``z``, ``v`` [B, T, C] (float32, bfloat16 or
+    float16; dense last dimension, any strides in front of it): the GRU update of the scans above with gates that do not read
+    the state, parallel in time.
+
+    ``h0`` [B, C] float32: state in front of step 0 (None: zero).  ``begin`` [B] int32: front padding, steps t < begin[b] leave
+    the state as it is and z, v are not looked at there.  ``period``: every period-th state is handed on (code/hpmn.py:124-128).
+    Returns (y [B, T/period, C] in z's dtype, h_last [B, C] float32, saved): ``saved`` is what ``gated_scan_bwd`` needs (None
+    unless ``train``)."""
+    B, T, Cc = _gated_scan_shape(z, v, begin, period)
+    dev = z.device
+    if h0 is not None:
+        _chk_seq("h0", h0, (B, Cc), torch.float32, dev)
+    y = torch.empty(B, T // period, Cc, device=dev, dtype=z.dtype)
+    h_last = torch.empty(B, Cc, device=dev, dtype=torch.float32)
+    tiles = -(-T // _lib.HPMN_GATED_SCAN_TILE)
+    saved = torch.empty(B, tiles, Cc, device=dev, dtype=torch.float32) if train else None
+    if h_last.numel() == 0:
+        return y, h_last, saved
+    if T == 0:
+        if h0 is None:
+            h_last.zero_()
+        else:
+            h_last.copy_(h0)
+        return y, h_last, saved
+    a = _lib.HpmnGatedScan()
+    a.B, a.T, a.C, a.dtype, a.period = B, T, Cc, _SEQ_DTYPES[z.dtype], period
+    a.z, a.v = z.data_ptr(), v.data_ptr()
+    a.z_sb, a.z_st, a.v_sb, a.v_st = z.stride(0), z.stride(1), v.stride(0), v.stride(1)
+    a.begin, a.h0 = _ptr(begin), _ptr(h0)
+    a.h0_sb = 0 if h0 is None else h0.stride(0)
+    a.y, a.y_sb, a.y_st, a.h_last, a.saved = y.data_ptr(), y.stride(0), y.stride(1), h_last.data_ptr(), _ptr(saved)
+    ws, a.workspace_bytes = _gated_scan_workspace(B, T, Cc, dev)
+    a.workspace = _ptr(ws)
+    _call_on(dev, "hpmn_gated_scan_fwd", _lib.load().hpmn_gated_scan_fwd, a)
+    return y, h_last, saved
+
+
+def gated_scan_bwd(z, v, saved, d_y, *, d_h_last=None, begin=None, period=1, out=None):
+    """hpmn_gated_scan_bwd: gradients of ``gated_scan_fwd`` (same ``z``, ``v``, ``begin``, ``period``; ``saved`` from its training
+    form).  ``d_y`` [B, T/period, C] in z's dtype or None, ``d_h_last`` [B, C] float32 or None.  ``out`` = (d_z, d_v): buffers to
+    write into, e.g. the halves of one projection's gradient (strided).  Returns (d_z, d_v, d_h0 float32 [B, C])."""
+    B, T, Cc = _gated_scan_shape(z, v, begin, period)
+    dev = z.device
+    tiles = -(-T // _lib.HPMN_GATED_SCAN_TILE)
+    if saved is None:
+        raise ValueError("saved: gated_scan_fwd has to run with train=True")
+    _chk_seq("saved", saved, (B, tiles, Cc), torch.float32, dev)
+    if not saved.is_contiguous():
+        raise ValueError("saved: expected the forward's own tensor")
+    if d_y is not None:
+        _chk_seq("d_y", d_y, (B, T // period, Cc), z.dtype, dev)
+    if d_h_last is not None:
+        _chk_seq("d_h_last", d_h_last, (B, Cc), torch.float32, dev)
+        d_h_last = d_h_last.contiguous()
+    if out is not None:
+        d_z, d_v = out
+        for n, t in (("d_z", d_z), ("d_v", d_v)):
+            _chk_seq(n, t, (B, T, Cc), z.dtype, dev)
+            _chk_out(n, t)
+    else:
+        d_z = torch.empty(B, T, Cc, device=dev, dtype=z.dtype)
+        d_v = torch.empty(B, T, Cc, device=dev, dtype=z.dtype)
+    d_h0 = torch.empty(B, Cc, device=dev, dtype=torch.float32)
+    if d_h0.numel() == 0:
+        return d_z, d_v, d_h0
+    if T == 0:
+        if d_h_last is None:
+            d_h0.zero_()
+        else:
+            d_h0.copy_(d_h_last)
+        return d_z, d_v, d_h0
+    a = _lib.HpmnGatedScanBwd()
+    a.B, a.T, a.C, a.dtype, a.period = B, T, Cc, _SEQ_DTYPES[z.dtype], period
+    a.z, a.v = z.data_ptr(), v.data_ptr()
+    a.z_sb, a.z_st, a.v_sb, a.v_st = z.stride(0), z.stride(1), v.stride(0), v.stride(1)
+    a.begin, a.saved, a.d_h_last = _ptr(begin), saved.data_ptr(), _ptr(d_h_last)
+    if d_y is not None:
+        a.d_y, a.dy_sb, a.dy_st = d_y.data_ptr(), d_y.stride(0), d_y.stride(1)
+    a.d_z, a.d_v, a.d_h0 = d_z.data_ptr(), d_v.data_ptr(), d_h0.data_ptr()
+    a.dz_sb, a.dz_st, a.dv_sb, a.dv_st = d_z.stride(0), d_z.stride(1), d_v.stride(0), d_v.stride(1)
+    ws, a.workspace_bytes = _gated_scan_workspace(B, T, Cc, dev)
+    a.workspace = _ptr(ws)
+    _call_on(dev, "hpmn_gated_scan_bwd", _lib.load().hpmn_gated_scan_bwd, a)
+    return d_z, d_v, d_h0
+
+
+def gated_scan_step(z, v, state, user=None, *, commit=True):
+    """hpmn_gated_scan_step: one event per row against stored states, the serving form of ``gated_scan_fwd``.  ``z``, ``v`` [B, C];
+    ``state`` [n_users, C] float32; ``user`` [B] int32 / int64 names every row's state (None: row b works on state b).  Returns y
+    [B, C] in z's dtype, the states after the event.
+
+    ``commit``: the new states are written to the store; events of the same user are applied in row order.  Without it the store
+    is only read (a candidate event scored as if it were the next one; any user may be named any number of times).  A row whose
+    user is outside the store changes nothing and gets NaN."""
+    _seq_input("z", z, 2)
+    B, Cc = z.shape
+    dev = z.device
+    _chk_seq("z", z, (B, Cc), z.dtype, dev)
+    _chk_seq("v", v, (B, Cc), z.dtype, dev)
+    if state.dim() != 2:
+        raise ValueError("state: expected [n_users, %d], got %s" % (Cc, tuple(state.shape)))
+    _chk_seq("state", state, (state.shape[0], Cc), torch.float32, dev)
+    _chk_out("state", state)
+    if user is None:
+        if state.shape[0] != B:
+            raise ValueError("%d rows against %d states: pass user" % (B, state.shape[0]))
+    elif not (user.device == dev and user.dtype in (torch.int32, torch.int64) and tuple(user.shape) == (B,) and user.is_contiguous()):
+        raise ValueError("user: expected contiguous int32 or int64 [%d] on %s, got %s %s" % (B, dev, user.dtype, tuple(user.shape)))
+    y = torch.empty(B, Cc, device=dev, dtype=z.dtype)
+    if y.numel() == 0:
+        return y
+    a = _lib.HpmnGatedStep()
+    a.C, a.dtype = Cc, _SEQ_DTYPES[z.dtype]
+    a.z_s, a.v_s, a.y_s = z.stride(0), v.stride(0), y.stride(0)
+    a.state, a.state_s, a.n_users = state.data_ptr(), max(state.stride(0), Cc), state.shape[0]
+    a.flags = (_lib.HPMN_STEP_COMMIT if commit else 0) | (_lib.HPMN_STEP_USER_I64 if user is not None and user.dtype == torch.int64 else 0)
+    # the ordered form works through its user list in calls of HPMN_STEP_MAX_INDEXED rows (one stream: still in row order)
+    step = _lib.HPMN_STEP_MAX_INDEXED if commit and user is not None else B
+    for lo in range(0, B, step):
+        a.B = min(step, B - lo)
+        a.z, a.v, a.y = z[lo:].data_ptr(), v[lo:].data_ptr(), y[lo:].data_ptr()
+        a.user = None if user is None else user[lo:].data_ptr()
+        _call_on(dev, "hpmn_gated_scan_step", _lib.load().hpmn_gated_scan_step, a)
+    return y

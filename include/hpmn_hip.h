@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define HPMN_ABI_VERSION 14
+#define HPMN_ABI_VERSION 15
 #define HPMN_ID_MASK0 1   /* id-flags bit 0: id 0 gathers a zero row and receives no gradient (the Hpmn class)  */
 #define HPMN_ID_I64 2     /* id-flags bit 1: the ids tensor is int64 (default: int32)                          */
 #define HPMN_ID_HOT 4     /* id-flags bit 2 (ABI v14; a HINT to the gradient scatter, ignored elsewhere): many lookups share
@@ -783,6 +783,88 @@ typedef struct HpmnOnlineUpdate {
 } HpmnOnlineUpdate;
 
 int hpmn_memory_update(const HpmnOnlineUpdate *args, void *stream);
+
+/* ------------------------------------------------------------------------------------
+ * Gated linear recurrence (ABI v15): the GRU update h = u h + (1 - u) c with gates and candidates that do NOT read the
+ * state, so that a layer over a lifelong sequence is parallel in time (a scan of affine maps) instead of a serial chain.
+ *
+ *   a_t = sigmoid(z_t),   h_t = a_t h_{t-1} + (1 - a_t) v_t,   y_j = h_{(j+1) period - 1}      j < T / period
+ *
+ * z, v: [B, T, C] of `dtype`; element strides over b and t are arguments (two halves of one projection buffer), the last
+ * dimension is dense.  States, gates and sums are fp32 whatever the dtype; y, d_z, d_v are rounded to it once.
+ *   begin  : optional [B] int32: front padding.  Steps t < begin[b] are identities (h_t = h_{t-1}, whatever z and v hold
+ *            there, NaN included) and have zero gradients; begin[b] >= T: nothing but padding.
+ *   h0     : optional [B, C] (row stride h0_sb): the state in front of step 0; NULL: zero.
+ *   y      : optional [B, T / period, C];  h_last: optional [B, C];  T % period == 0.
+ *   saved  : optional [B, ceil(T / HPMN_GATED_SCAN_TILE), C]: the state in front of every tile of HPMN_GATED_SCAN_TILE
+ *            steps, all that the backward needs of the forward besides z and v (it recomputes the states inside a tile).
+ * Backward, with G_t = dL/dh_t in full:
+ *   G_t = d_y[fires at t] + a_{t+1} G_{t+1}  (+ d_h_last at T-1);   d_v = (1-a) G;   d_z = G (h_{t-1} - v) a (1-a);
+ *   d_h0 = a_0 G_0.   Deterministic.  d_z / d_v / d_h0 are overwritten; d_y, d_h_last, d_h0 may be NULL (zero / not wanted).
+ * workspace: >= hpmn_gated_scan_workspace_bytes(B, T, C) bytes (16-byte aligned; may be 0 bytes: NULL then), used by this call only.
+ * ---------------------------------------------------------------------------------- */
+#define HPMN_F32 0
+#define HPMN_BF16 1
+#define HPMN_F16 2
+#define HPMN_GATED_SCAN_TILE 128
+
+typedef struct HpmnGatedScan {
+    int32_t B, T, C, dtype, period, pad_;
+    const void *z, *v;
+    int64_t z_sb, z_st, v_sb, v_st;
+    const int32_t *begin;
+    const float *h0;
+    int64_t h0_sb;
+    void *y;
+    int64_t y_sb, y_st;
+    float *h_last;          /* [B, C] dense */
+    float *saved;
+    void *workspace;
+    size_t workspace_bytes;
+} HpmnGatedScan;
+
+typedef struct HpmnGatedScanBwd {
+    int32_t B, T, C, dtype, period, pad_;
+    const void *z, *v;
+    int64_t z_sb, z_st, v_sb, v_st;
+    const int32_t *begin;
+    const float *saved;     /* as the forward of the same z, v, begin, h0 left it */
+    const void *d_y;
+    int64_t dy_sb, dy_st;
+    const float *d_h_last;  /* [B, C] dense */
+    void *d_z, *d_v;
+    int64_t dz_sb, dz_st, dv_sb, dv_st;
+    float *d_h0;            /* [B, C] dense */
+    void *workspace;
+    size_t workspace_bytes;
+} HpmnGatedScanBwd;
+
+size_t hpmn_gated_scan_workspace_bytes(int32_t B, int32_t T, int32_t C);
+int hpmn_gated_scan_fwd(const HpmnGatedScan *args, void *stream);
+int hpmn_gated_scan_bwd(const HpmnGatedScanBwd *args, void *stream);
+
+/* One event per row against stored states -- the serving form of the recurrence above.
+ *   z, v  : [B, C] rows (strides z_s, v_s);   state: [n_users, C] fp32 (row stride state_s);   y: optional [B, C] of `dtype`
+ *   user  : optional [B] int32 (int64 with HPMN_STEP_USER_I64): row b works on state[user[b]]; NULL: on state[b], B == n_users.
+ *           A row whose index is outside [0, n_users) leaves the store alone and gets y = NaN.
+ *   HPMN_STEP_COMMIT: the new state is written to the store.  Rows that name the same user are then applied in row order
+ *           (each sees the state the one before it left); at most HPMN_STEP_MAX_INDEXED rows with `user` in that form.
+ *   without it: the store is read only -- a candidate event scored "as if it were the next one"; rows are independent. */
+#define HPMN_STEP_COMMIT 1
+#define HPMN_STEP_USER_I64 2
+#define HPMN_STEP_MAX_INDEXED 4096
+typedef struct HpmnGatedStep {
+    int32_t B, C, dtype, flags;
+    const void *z, *v;
+    int64_t z_s, v_s;
+    float *state;
+    int64_t state_s, n_users;
+    const void *user;
+    void *y;
+    int64_t y_s;
+} HpmnGatedStep;
+
+int hpmn_gated_scan_step(const HpmnGatedStep *args, void *stream);
 
 #ifdef __cplusplus
 }
