@@ -237,7 +237,14 @@ class HpmnGatedStep(C.Structure):
                 ("user", C.c_void_p), ("y", C.c_void_p), ("y_s", C.c_int64)]
 
 
+class HpmnDropout(C.Structure):
+    _fields_ = [("N", C.c_int64), ("C", C.c_int64), ("dtype", C.c_int32), ("keep_prob", C.c_float), ("x", C.c_void_p),
+                ("residual", C.c_void_p), ("y", C.c_void_p), ("x_s", C.c_int64), ("r_s", C.c_int64), ("y_s", C.c_int64),
+                ("seed", C.c_uint64), ("offset", C.c_uint64), ("rng", C.c_void_p)]
+
+
 SIGNATURES = {
+    "hpmn_dropout": (C.c_int, [C.POINTER(HpmnDropout), C.c_void_p]),
     "hpmn_gated_scan_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32]),
     "hpmn_gated_scan_fwd": (C.c_int, [C.POINTER(HpmnGatedScan), C.c_void_p]),
     "hpmn_gated_scan_bwd": (C.c_int, [C.POINTER(HpmnGatedScanBwd), C.c_void_p]),

@@ -7,6 +7,7 @@ size_t gated_scan_workspace_bytes(int B, int T, int C);
 int gated_scan_fwd_launch(const HpmnGatedScan &a, hipStream_t st);
 int gated_scan_bwd_launch(const HpmnGatedScanBwd &a, hipStream_t st);
 int gated_step_launch(const HpmnGatedStep &a, hipStream_t st);
+int dropout_launch(const HpmnDropout &a, unsigned threshold, hipStream_t st);
 
 static inline bool known_dtype(int d) { return d == HPMN_F32 || d == HPMN_BF16 || d == HPMN_F16; }
 static inline bool aligned_to(const void *p, int dtype) { return is_aligned(p, elem_size(dtype)); }
@@ -72,6 +73,22 @@ int hpmn_gated_scan_step(const HpmnGatedStep *a, void *stream) {
     if (a->user && (a->flags & HPMN_STEP_COMMIT) && a->B > HPMN_STEP_MAX_INDEXED) return HPMN_EUNSUPPORTED;
     if ((long)a->B * ((a->C + 3) / 4) >= (1l << 36)) return HPMN_EUNSUPPORTED;
     return gated_step_launch(*a, (hipStream_t)stream);
+}
+
+int hpmn_dropout(const HpmnDropout *a, void *stream) {
+    drop_stale_hip_error();
+    if (!a) return HPMN_EINVAL;
+    if (a->N < 0 || a->C < 0 || !known_dtype(a->dtype) || !(a->keep_prob > 0.f && a->keep_prob <= 1.f)) return HPMN_EINVAL;
+    if (a->N == 0 || a->C == 0) return HPMN_OK;
+    if (!a->x || !a->y) return HPMN_EINVAL;
+    if (!aligned_to(a->x, a->dtype) || !aligned_to(a->y, a->dtype) || !aligned_to(a->residual, a->dtype)) return HPMN_EINVAL;
+    if (!is_aligned(a->rng, 8)) return HPMN_EINVAL;
+    if (a->x_s < 0 || a->r_s < 0 || (a->N > 1 && a->y_s < a->C)) return HPMN_EINVAL;
+    if (a->N > (1l << 40) / a->C) return HPMN_EUNSUPPORTED;      // one launch: blocks of 2048 elements in a 31-bit grid
+    // floor(p 2^16 + 1/2), as a double: p is a float, so the product is exact
+    const double q = (double)a->keep_prob * 65536.0 + 0.5;
+    const unsigned thr = q < 1.0 ? 1u : (unsigned)q;
+    return dropout_launch(*a, thr > 65536u ? 65536u : thr, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -1753,3 +1753,46 @@ def gated_scan_step(z, v, state, user=None, *, commit=True):
         a.user = None if user is None else user[lo:].data_ptr()
         _call_on(dev, "hpmn_gated_scan_step", _lib.load().hpmn_gated_scan_step, a)
     return y
+
+
+def _dropout(name, x, keep_prob, seed, offset, residual, rng):
+    if x.dim() == 0:
+        raise ValueError("%s: a tensor of at least one dimension" % name)
+    _seq_input("x", x, x.dim())
+    if not 0.0 < keep_prob <= 1.0:
+        raise ValueError("keep_prob has to be in (0, 1], got %r" % (keep_prob,))
+    dev, shape = x.device, x.shape
+    if rng is not None and not (rng.device == dev and rng.dtype == torch.int64 and tuple(rng.shape) == (2,) and rng.is_contiguous()):
+        raise ValueError("rng: expected contiguous int64 [2] on %s" % dev)
+    if residual is not None:
+        _chk_seq("residual", residual, shape, x.dtype, dev)
+    y = torch.empty(shape, device=dev, dtype=x.dtype)
+    if y.numel() == 0:
+        return y
+    Cc = shape[-1]
+    # 2-D views: rows at one stride.  What cannot be viewed that way (a permuted tensor) is copied into order first.
+    rows = [None if t is None else t.reshape(-1, Cc) for t in (x, residual)]
+    rows = [t if t is None or Cc == 1 or t.stride(1) == 1 else t.contiguous() for t in rows]
+    a = _lib.HpmnDropout()
+    a.N, a.C, a.dtype, a.keep_prob = y.numel() // Cc, Cc, _SEQ_DTYPES[x.dtype], keep_prob
+    a.x, a.x_s, a.y, a.y_s = rows[0].data_ptr(), rows[0].stride(0), y.data_ptr(), Cc
+    if residual is not None:
+        a.residual, a.r_s = rows[1].data_ptr(), rows[1].stride(0)
+    a.seed, a.offset, a.rng = seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _ptr(rng)
+    _call_on(dev, "hpmn_dropout", _lib.load().hpmn_dropout, a)
+    return y
+
+
+def dropout_fwd(x, keep_prob, seed, *, offset=0, residual=None, rng=None):
+    """hpmn_dropout: y = x * keep / p (+ ``residual``) with keep decisions from a counter-based generator (no mask is stored).
+    Element i of x in row-major order is kept iff 16-bit field i % 4 of splitmix64 word (seed, ``offset`` + i / 4) is below
+    round(keep_prob * 65536); a call uses ceil(x.numel() / 4) counters, the next call's ``offset`` starts behind them.
+
+    ``x`` float32 / bfloat16 / float16, any shape; ``rng``: int64 [2] on the device, {seed, offset}: replaces ``seed`` and is added to
+    ``offset`` when the kernel runs, so that a captured graph draws anew after the caller has advanced it."""
+    return _dropout("dropout_fwd", x, keep_prob, seed, offset, residual, rng)
+
+
+def dropout_bwd(d_y, keep_prob, seed, *, offset=0, rng=None):
+    """Gradient wrt x of ``dropout_fwd`` under the same keep_prob / seed / offset / rng values (the residual's gradient is d_y)."""
+    return _dropout("dropout_bwd", d_y, keep_prob, seed, offset, None, rng)

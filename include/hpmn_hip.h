@@ -866,6 +866,33 @@ typedef struct HpmnGatedStep {
 
 int hpmn_gated_scan_step(const HpmnGatedStep *args, void *stream);
 
+/* ------------------------------------------------------------------------------------
+ * Dropout with keep decisions from a counter-based generator: y = keep * x / p (+ residual), no mask in memory; the
+ * backward is the same call on d_y.  (The read path draws its head's masks the same way inside hpmn_read_fwd_bwd.)
+ *   Element i = row * C + column of the [N, C] tensor is kept iff field i % 4 (16 bits, low first) of
+ *       word(i / 4) = mix(mix(seed) + 0x9E3779B97F4A7C15 * (offset + i / 4 + 1))
+ *   is below thr = round(keep_prob * 65536) (at least 1), mix = splitmix64's output function (Steele, Lea, Flood 2014):
+ *       x ^= x >> 30; x *= 0xBF58476D1CE4E5B9; x ^= x >> 27; x *= 0x94D049BB133111EB; x ^= x >> 31   (mod 2^64).
+ *   Kept elements are scaled by 65536 / thr, so the expectation is exact for the quantised probability.  A call uses the counters
+ *   [offset, offset + ceil(N C / 4)); seeds are mixed, so neighbouring seeds have unrelated streams.
+ *   rng    : optional 2 device uint64 {seed, offset}: used as seed = rng[0], offset += rng[1] (read by the kernel: a
+ *            captured graph draws anew when the caller advances them between replays).
+ *   x, residual (optional), y: [N, C] of dtype, row strides x_s / r_s / y_s in elements, dense columns.  y == x and
+ *            y == residual are fine.  fp32 arithmetic, rounded once.
+ * ---------------------------------------------------------------------------------- */
+typedef struct HpmnDropout {
+    int64_t N, C;
+    int32_t dtype;
+    float keep_prob;        /* (0, 1] */
+    const void *x, *residual;
+    void *y;
+    int64_t x_s, r_s, y_s;
+    uint64_t seed, offset;
+    const uint64_t *rng;
+} HpmnDropout;
+
+int hpmn_dropout(const HpmnDropout *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
