@@ -243,7 +243,20 @@ class HpmnDropout(C.Structure):
                 ("seed", C.c_uint64), ("offset", C.c_uint64), ("rng", C.c_void_p)]
 
 
+class HpmnPrefixAttn(C.Structure):
+    _fields_ = ([(f, C.c_int32) for f in ("B", "Lq", "Hq", "Hkv", "D", "dtype", "P", "S")] + [("scale", C.c_float), ("pad_", C.c_int32)] +
+                [("q", C.c_void_p)] + [(f, C.c_int64) for f in ("q_sb", "q_sl", "q_sh")] +
+                [("k_pre", C.c_void_p), ("v_pre", C.c_void_p)] + [(f, C.c_int64) for f in ("kp_st", "kp_sh", "vp_st", "vp_sh")] +
+                [("k_suf", C.c_void_p), ("v_suf", C.c_void_p)] +
+                [(f, C.c_int64) for f in ("ks_sb", "ks_st", "ks_sh", "vs_sb", "vs_st", "vs_sh")] +
+                [("prefix_len", C.c_void_p), ("suffix_len", C.c_void_p), ("out", C.c_void_p)] +
+                [(f, C.c_int64) for f in ("o_sb", "o_sl", "o_sh")] +
+                [("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)])
+
+
 SIGNATURES = {
+    "hpmn_prefix_attn_workspace_bytes": (C.c_size_t, [C.POINTER(HpmnPrefixAttn)]),
+    "hpmn_prefix_attn": (C.c_int, [C.POINTER(HpmnPrefixAttn), C.c_void_p]),
     "hpmn_dropout": (C.c_int, [C.POINTER(HpmnDropout), C.c_void_p]),
     "hpmn_gated_scan_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32]),
     "hpmn_gated_scan_fwd": (C.c_int, [C.POINTER(HpmnGatedScan), C.c_void_p]),

@@ -7,6 +7,8 @@ size_t gated_scan_workspace_bytes(int B, int T, int C);
 int gated_scan_fwd_launch(const HpmnGatedScan &a, hipStream_t st);
 int gated_scan_bwd_launch(const HpmnGatedScanBwd &a, hipStream_t st);
 int gated_step_launch(const HpmnGatedStep &a, hipStream_t st);
+size_t prefix_attn_workspace_bytes(const HpmnPrefixAttn &a);
+int prefix_attn_launch(const HpmnPrefixAttn &a, hipStream_t st);
 int dropout_launch(const HpmnDropout &a, unsigned threshold, hipStream_t st);
 
 static inline bool known_dtype(int d) { return d == HPMN_F32 || d == HPMN_BF16 || d == HPMN_F16; }
@@ -14,6 +16,15 @@ static inline bool aligned_to(const void *p, int dtype) { return is_aligned(p, e
 
 // One grid dimension and 32-bit block indices: (sequences) x (channel blocks) has to stay below 2^31.
 static inline bool scan_grid_ok(int B, int C) { return (long)B * ((C + 15) / 16) < (1l << 30); }
+
+// Sizes that every index of the attention kernels fits: query rows, keys and work items in 31 bits, head groups whole.
+static inline int prefix_attn_sizes(const HpmnPrefixAttn &a) {
+    if (a.B < 0 || a.Lq < 0 || a.Hq < 1 || a.Hkv < 1 || a.D < 1 || a.P < 0 || a.S < 0 || a.Hq % a.Hkv != 0 || !known_dtype(a.dtype))
+        return HPMN_EINVAL;
+    if (a.D > 128 || a.P > (1 << 30) || a.S > (1 << 30)) return HPMN_EUNSUPPORTED;
+    if ((double)a.B * a.Lq * a.Hq > (double)(1 << 26)) return HPMN_EUNSUPPORTED;
+    return HPMN_OK;
+}
 
 }  // namespace hpmn
 
@@ -89,6 +100,32 @@ int hpmn_dropout(const HpmnDropout *a, void *stream) {
     const double q = (double)a->keep_prob * 65536.0 + 0.5;
     const unsigned thr = q < 1.0 ? 1u : (unsigned)q;
     return dropout_launch(*a, thr > 65536u ? 65536u : thr, (hipStream_t)stream);
+}
+
+size_t hpmn_prefix_attn_workspace_bytes(const HpmnPrefixAttn *a) {
+    if (!a || prefix_attn_sizes(*a) != HPMN_OK || a->B == 0 || a->Lq == 0) return 0;
+    return prefix_attn_workspace_bytes(*a);
+}
+
+int hpmn_prefix_attn(const HpmnPrefixAttn *a, void *stream) {
+    drop_stale_hip_error();
+    if (!a) return HPMN_EINVAL;
+    const int rc = prefix_attn_sizes(*a);
+    if (rc != HPMN_OK) return rc;
+    if (a->B == 0 || a->Lq == 0) return HPMN_OK;
+    if (!a->q || !a->out || (a->P > 0 && (!a->k_pre || !a->v_pre)) || (a->S > 0 && (!a->k_suf || !a->v_suf))) return HPMN_EINVAL;
+    const void *typed[] = {a->q, a->k_pre, a->v_pre, a->k_suf, a->v_suf, a->out};
+    for (const void *p : typed)
+        if (!aligned_to(p, a->dtype)) return HPMN_EINVAL;
+    if (!is_aligned(a->lse, 4) || !is_aligned(a->prefix_len, 4) || !is_aligned(a->suffix_len, 4)) return HPMN_EINVAL;
+    const int64_t strides[] = {a->q_sb, a->q_sl, a->q_sh, a->kp_st, a->kp_sh, a->vp_st, a->vp_sh, a->ks_sb, a->ks_st,
+                               a->ks_sh, a->vs_sb, a->vs_st, a->vs_sh, a->o_sb, a->o_sl, a->o_sh};
+    for (int64_t s : strides)
+        if (s < 0) return HPMN_EINVAL;
+    if (!(a->scale - a->scale == 0.f)) return HPMN_EINVAL;                       // infinite or NaN
+    const size_t need = prefix_attn_workspace_bytes(*a);
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need || !is_aligned(a->workspace, 16))) return HPMN_EINVAL;
+    return prefix_attn_launch(*a, (hipStream_t)stream);
 }
 
 }  // extern "C"

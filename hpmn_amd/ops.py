@@ -1796,3 +1796,64 @@ def dropout_fwd(x, keep_prob, seed, *, offset=0, residual=None, rng=None):
 def dropout_bwd(d_y, keep_prob, seed, *, offset=0, rng=None):
     """Gradient wrt x of ``dropout_fwd`` under the same keep_prob / seed / offset / rng values (the residual's gradient is d_y)."""
     return _dropout("dropout_bwd", d_y, keep_prob, seed, offset, None, rng)
+
+
+def shared_prefix_attention(q, k_prefix, v_prefix, k_suffix=None, v_suffix=None, *, prefix_len=None, suffix_len=None, scale=None,
+                            want_lse=False):
+    """hpmn_prefix_attn: softmax attention of a batch whose rows share a long prefix (many candidates against one history; the
+    prefix is read once for the whole batch).  ``q`` [B, Lq, Hq, D], ``k_prefix`` / ``v_prefix`` [P, Hkv, D], ``k_suffix`` /
+    ``v_suffix`` [B, S, Hkv, D] or None: keys of every row's own; float32 / bfloat16 / float16, D <= 128, Hq a multiple of Hkv,
+    dense last dimension.
+
+    ``prefix_len``: int32 [1] on the device, the prefix in use (None: P).  ``suffix_len``: int32 [B] (None: S); with several query
+    tokens they are the last of the suffix and see it up to their own position.  ``scale``: default D ** -0.5.  Returns out
+    [B, Lq, Hq, D] (a query without any key: zeros), with ``want_lse`` also the log-sum-exp [B, Lq, Hq] float32 (-inf there)."""
+    dt = _seq_input("q", q, 4)
+    B, Lq, Hq, D = q.shape
+    dev = q.device
+    _chk_seq("q", q, q.shape, q.dtype, dev)
+    if k_prefix.dim() != 3:
+        raise ValueError("k_prefix: expected [P, Hkv, D], got %s" % (tuple(k_prefix.shape),))
+    P, Hkv = k_prefix.shape[:2]
+    if Hkv < 1 or Hq < 1 or D < 1 or Hq % Hkv != 0:
+        raise ValueError("%d query heads of %d over %d key heads" % (Hq, D, Hkv))
+    if D > 128:
+        raise ValueError("head dimension %d: at most 128" % D)
+    _chk_seq("k_prefix", k_prefix, (P, Hkv, D), q.dtype, dev)
+    _chk_seq("v_prefix", v_prefix, (P, Hkv, D), q.dtype, dev)
+    if (k_suffix is None) != (v_suffix is None):
+        raise ValueError("k_suffix and v_suffix go together")
+    S = 0
+    if k_suffix is not None:
+        if k_suffix.dim() != 4:
+            raise ValueError("k_suffix: expected [B, S, Hkv, D], got %s" % (tuple(k_suffix.shape),))
+        S = k_suffix.shape[1]
+        _chk_seq("k_suffix", k_suffix, (B, S, Hkv, D), q.dtype, dev)
+        _chk_seq("v_suffix", v_suffix, (B, S, Hkv, D), q.dtype, dev)
+    for name, t, n in (("prefix_len", prefix_len, 1), ("suffix_len", suffix_len, B)):
+        if t is not None and not (t.device == dev and t.dtype == torch.int32 and tuple(t.shape) == (n,) and t.is_contiguous()):
+            raise ValueError("%s: expected contiguous int32 [%d] on %s, got %s %s" % (name, n, dev, t.dtype, tuple(t.shape)))
+    if scale is None:
+        scale = D ** -0.5
+    if not math.isfinite(scale):
+        raise ValueError("scale has to be finite, got %r" % (scale,))
+    out = torch.empty(B, Lq, Hq, D, device=dev, dtype=q.dtype)
+    lse = torch.empty(B, Lq, Hq, device=dev, dtype=torch.float32) if want_lse else None
+    if out.numel() > 0:
+        a = _lib.HpmnPrefixAttn()
+        a.B, a.Lq, a.Hq, a.Hkv, a.D, a.dtype, a.P, a.S, a.scale = B, Lq, Hq, Hkv, D, dt, P, S, scale
+        a.q, a.q_sb, a.q_sl, a.q_sh = q.data_ptr(), q.stride(0), q.stride(1), q.stride(2)
+        a.k_pre, a.kp_st, a.kp_sh = k_prefix.data_ptr(), k_prefix.stride(0), k_prefix.stride(1)
+        a.v_pre, a.vp_st, a.vp_sh = v_prefix.data_ptr(), v_prefix.stride(0), v_prefix.stride(1)
+        if S:
+            a.k_suf, a.ks_sb, a.ks_st, a.ks_sh = (k_suffix.data_ptr(),) + k_suffix.stride()[:3]
+            a.v_suf, a.vs_sb, a.vs_st, a.vs_sh = (v_suffix.data_ptr(),) + v_suffix.stride()[:3]
+        a.prefix_len, a.suffix_len = _ptr(prefix_len), _ptr(suffix_len)
+        a.out, a.o_sb, a.o_sl, a.o_sh, a.lse = out.data_ptr(), out.stride(0), out.stride(1), out.stride(2), _ptr(lse)
+        lib = _lib.load()
+        a.workspace_bytes = lib.hpmn_prefix_attn_workspace_bytes(C.byref(a))
+        # per call: the caching allocator keeps it on the call's stream, and a captured graph owns its own
+        ws = torch.empty(a.workspace_bytes, device=dev, dtype=torch.uint8) if a.workspace_bytes else None
+        a.workspace = _ptr(ws)
+        _call_on(dev, "hpmn_prefix_attn", lib.hpmn_prefix_attn, a)
+    return (out, lse) if want_lse else out

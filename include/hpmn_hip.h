@@ -893,6 +893,41 @@ typedef struct HpmnDropout {
 
 int hpmn_dropout(const HpmnDropout *args, void *stream);
 
+/* ------------------------------------------------------------------------------------
+ * Attention of a batch whose rows share a long prefix (serving: many candidates against ONE history): every query token
+ * attends to the P shared keys, which are read once for the whole batch instead of once per row, and to the visible
+ * keys of its own row's suffix.
+ *   q   [B, Lq, Hq, D]        k_pre, v_pre [P, Hkv, D]        k_suf, v_suf [B, S, Hkv, D] (S == 0: NULL)
+ *   out [B, Lq, Hq, D] = softmax over both of scale q . k, times v;   lse (optional) [B, Lq, Hq] fp32: log of the sum of exp
+ * Query head h reads key head h / (Hq / Hkv).  Rows of D elements are dense, all other strides (in elements) are arguments.
+ *   prefix_len : optional, ONE device int32: the prefix in use, clamped to [0, P] (a captured graph follows it); NULL: P
+ *   suffix_len : optional [B] device int32, clamped to [0, S]; NULL: S.  The Lq query tokens are the suffix's last: token i sees
+ *                suffix keys j < suffix_len - Lq + 1 + i (one query token: all of them) and the whole prefix.
+ * Keys and values behind the lengths are not looked at.  A query that sees no key at all gets out = 0, lse = -inf.
+ * D <= 128.  Scores, maxima, sums and the output accumulator are fp32 for every dtype.
+ * workspace: >= hpmn_prefix_attn_workspace_bytes(args) bytes (16-byte aligned; the size depends on the sizes alone).
+ * ---------------------------------------------------------------------------------- */
+typedef struct HpmnPrefixAttn {
+    int32_t B, Lq, Hq, Hkv, D, dtype, P, S;
+    float scale;
+    int32_t pad_;
+    const void *q;
+    int64_t q_sb, q_sl, q_sh;
+    const void *k_pre, *v_pre;
+    int64_t kp_st, kp_sh, vp_st, vp_sh;
+    const void *k_suf, *v_suf;
+    int64_t ks_sb, ks_st, ks_sh, vs_sb, vs_st, vs_sh;
+    const int32_t *prefix_len, *suffix_len;
+    void *out;
+    int64_t o_sb, o_sl, o_sh;
+    float *lse;             /* dense */
+    void *workspace;
+    size_t workspace_bytes;
+} HpmnPrefixAttn;
+
+size_t hpmn_prefix_attn_workspace_bytes(const HpmnPrefixAttn *args);
+int hpmn_prefix_attn(const HpmnPrefixAttn *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
