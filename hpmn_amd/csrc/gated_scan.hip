@@ -1,74 +1,294 @@
 // Gated linear recurrence (include/hpmn_hip.h): h_t = a_t h_{t-1} + (1 - a_t) v_t with a = sigmoid(z), forward, backward and
 // the one-event step.
 //
-// First form: one lane per (sequence, channel), the time loop serial in it.
+// h -> a h + u v are affine maps, their composition is associative: (A2, B2) o (A1, B1) = (A2 A1, A2 B1 + B2).  A workgroup owns
+// one sequence and a block of channels and walks the time axis in tiles of 128 steps held in registers:
+//   lane = (4 channels) x (a run of 4 consecutive steps): composes its run, 16-byte accesses in fp32, 8-byte in bf16 / fp16;
+//   the runs of a wave are scanned with lane shuffles, the waves of a tile through LDS (one barrier per tile, two buffers);
+//   the carried state enters, the run is replayed from it and stored.
+// z and v are read once, y is written once, nothing else reaches memory (training: one fp32 row per tile and channel).  Bound
+// by memory: the next tile's rows are in flight while this one is composed.
+// The backward walks the tiles in reverse.  Its scan G -> a (G + d_y) has the SAME a as the forward's, so one exchange serves
+// both: the states are recomputed from the tile's saved first row instead of being stored (a read of z and v, which d_z and d_v
+// need anyway, against a write and a read of all states in fp32).
+#include <algorithm>
+
 #include "seq_types.h"
 
 namespace hpmn {
 
 constexpr int TILE = HPMN_GATED_SCAN_TILE;
+constexpr int RUN = 4;                       // steps per lane and tile
+constexpr int MAX_WAVES = 8;                 // TILE = waves * (64 / LPR) * RUN
 
-template <typename T>
-__global__ __launch_bounds__(64) void gated_scan_fwd_kernel(const HpmnGatedScan a) {
-    const int nc = (a.C + 63) / 64;
-    const long b = blockIdx.x / nc;
-    const int c = (blockIdx.x % nc) * 64 + threadIdx.x;
-    if (c >= a.C) return;
-    const T *z = (const T *)a.z + b * a.z_sb + c, *v = (const T *)a.v + b * a.v_sb + c;
-    const int begin = a.begin ? a.begin[b] : 0;
-    const int tiles = (a.T + TILE - 1) / TILE;
-    float h = a.h0 ? a.h0[b * a.h0_sb + c] : 0.f;
-    for (int t = 0; t < a.T; ++t) {
-        if (a.saved && t % TILE == 0) a.saved[(b * tiles + t / TILE) * a.C + c] = h;
-        if (t >= begin) {
-            float ag, ug;
-            gate_pair((float)z[t * a.z_st], ag, ug);
-            h = fmaf(ag, h, ug * (float)v[t * a.v_st]);
-        }
-        if (a.y && (t + 1) % a.period == 0) ((T *)a.y)[b * a.y_sb + ((t + 1) / a.period - 1) * a.y_st + c] = (T)h;
-    }
-    if (a.h_last) a.h_last[b * a.C + c] = h;
+// barrier that orders LDS alone: __syncthreads() would also wait for the tile's stores to reach memory
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ v4f shfl_up4(v4f x, int d) {
+    v4f r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __shfl_up(x[i], d);
+    return r;
+}
+__device__ __forceinline__ v4f shfl_down4(v4f x, int d) {
+    v4f r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __shfl_down(x[i], d);
+    return r;
+}
+__device__ __forceinline__ v4f load_state(const float *p, int n) {          // n channels of a dense fp32 row
+    v4f r = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < n) r[i] = p[i];
+    return r;
+}
+__device__ __forceinline__ void store_state(float *p, v4f x, int n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < n) p[i] = x[i];
 }
 
+// Which steps fire (t + 1 a multiple of the period), and the row they fire into, kept without a division per step.
+struct Firing {
+    int q, r, period;
+    __device__ __forceinline__ void start(int t, int p) { period = p; q = t / p; r = t - q * p; }
+    __device__ __forceinline__ void jump(int dq, int dr) {                  // by dq * period + dr steps, |dr| < period
+        q += dq;
+        r += dr;
+        if (r >= period) { r -= period; ++q; }
+        else if (r < 0) { r += period; --q; }
+    }
+};
+
+// z, v: dense channels at row strides; one lane's run of RUN steps from step t on, only steps in [lo, hi) are touched.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_run(quad_t<T> (&q)[RUN], const T *p, long stride, int t, int lo, int hi, int n) {
+#pragma unroll
+    for (int s = 0; s < RUN; ++s) {
+        q[s] = quad_t<T>{};
+        if (t + s >= lo && t + s < hi) q[s] = load_quad<T, VEC>(p + (long)(t + s) * stride, n);
+    }
+}
+
+// a and u of a run; steps outside [lo, hi) are the identity (a = 1, u = 0, whatever was or was not loaded).
 template <typename T>
-__global__ __launch_bounds__(64) void gated_scan_bwd_kernel(const HpmnGatedScanBwd a) {
-    __shared__ float hs[TILE][64];           // the states in front of every step of a tile (a column per lane)
-    const int nc = (a.C + 63) / 64;
-    const long b = blockIdx.x / nc;
-    const int lane = threadIdx.x, c = (blockIdx.x % nc) * 64 + lane;
-    if (c >= a.C) return;
-    const T *z = (const T *)a.z + b * a.z_sb + c, *v = (const T *)a.v + b * a.v_sb + c;
-    const int begin = a.begin ? a.begin[b] : 0;
-    const int tiles = (a.T + TILE - 1) / TILE;
-    float G = a.d_h_last ? a.d_h_last[b * a.C + c] : 0.f;
-    for (int k = tiles - 1; k >= 0; --k) {
-        const int t0 = k * TILE, n = min(TILE, a.T - t0);
-        float h = a.saved[(b * tiles + k) * a.C + c];
-        for (int i = 0; i < n; ++i) {
-            hs[i][lane] = h;
-            if (t0 + i >= begin) {
-                float ag, ug;
-                gate_pair((float)z[(t0 + i) * a.z_st], ag, ug);
-                h = fmaf(ag, h, ug * (float)v[(t0 + i) * a.v_st]);
-            }
-        }
-        for (int i = n - 1; i >= 0; --i) {
-            const long t = t0 + i;
-            if (a.d_y && (t + 1) % a.period == 0)
-                G += (float)((const T *)a.d_y)[b * a.dy_sb + ((t + 1) / a.period - 1) * a.dy_st + c];
-            float dz = 0.f, dv = 0.f;
-            if (t >= begin) {
-                float ag, ug;
-                gate_pair((float)z[t * a.z_st], ag, ug);
-                dv = ug * G;
-                dz = ag * dv * (hs[i][lane] - (float)v[t * a.v_st]);
-                G *= ag;
-            }
-            ((T *)a.d_z)[b * a.dz_sb + t * a.dz_st + c] = (T)dz;
-            ((T *)a.d_v)[b * a.dv_sb + t * a.dv_st + c] = (T)dv;
+__device__ __forceinline__ void gate_run(const quad_t<T> (&zr)[RUN], int t, int lo, int hi, v4f (&ag)[RUN], v4f (&ug)[RUN]) {
+#pragma unroll
+    for (int s = 0; s < RUN; ++s) {
+        const bool live = t + s >= lo && t + s < hi;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x, y;
+            gate_pair((float)zr[s][i], x, y);
+            ag[s][i] = live ? x : 1.f;
+            ug[s][i] = live ? y : 0.f;
         }
     }
-    if (a.d_h0) a.d_h0[b * a.C + c] = G;
+}
+
+template <typename T, int LPR, bool VEC>
+__global__ __launch_bounds__(512) void gated_scan_fwd_kernel(const HpmnGatedScan a) {
+    constexpr int TG = 64 / LPR;             // runs side by side in a wave
+    __shared__ v4f agg[2][MAX_WAVES][2][LPR];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    const int cg = lane % LPR, tg = lane / LPR;
+    const int ncb = (a.C + 4 * LPR - 1) / (4 * LPR);
+    const long b = blockIdx.x / ncb;
+    const int c = ((int)(blockIdx.x % ncb) * LPR + cg) * 4;
+    const int n = max(0, min(4, a.C - c));   // this lane's channels (0: none, it only takes part in the exchange)
+    const int step = nw * TG * RUN;          // steps per tile (TILE, or fewer when the whole sequence fits)
+    const int tiles = (a.T + TILE - 1) / TILE;
+    const int lo = n > 0 ? (a.begin ? a.begin[b] : 0) : a.T, hi = a.T;
+    const T *z = (const T *)a.z + b * a.z_sb + c, *v = (const T *)a.v + b * a.v_sb + c;
+    T *y = (T *)a.y + b * a.y_sb + c;
+    const long crow = b * a.C + c;
+
+    v4f carry = {0.f, 0.f, 0.f, 0.f};
+    if (a.h0) carry = load_state(a.h0 + b * a.h0_sb + c, n);
+    int t = (w * TG + tg) * RUN;
+    Firing f;
+    f.start(t, a.period);
+    const int dq = step / a.period, dr = step % a.period;
+    quad_t<T> zr[RUN], vr[RUN];
+    load_run<T, VEC>(zr, z, a.z_st, t, lo, hi, n);
+    load_run<T, VEC>(vr, v, a.v_st, t, lo, hi, n);
+    for (int k = 0, t0 = 0; t0 < a.T; ++k, t0 += step) {
+        v4f ag[RUN], bv[RUN];
+        gate_run<T>(zr, t, lo, hi, ag, bv);
+#pragma unroll
+        for (int s = 0; s < RUN; ++s) {
+            // (steps outside were not loaded: their v is zero)
+            bv[s] *= __builtin_convertvector(vr[s], v4f);
+        }
+        const int tn = t + step;
+        load_run<T, VEC>(zr, z, a.z_st, tn, lo, hi, n);
+        load_run<T, VEC>(vr, v, a.v_st, tn, lo, hi, n);
+        v4f A = ag[0], Bc = bv[0];
+#pragma unroll
+        for (int s = 1; s < RUN; ++s) {
+            Bc = ag[s] * Bc + bv[s];
+            A *= ag[s];
+        }
+#pragma unroll
+        for (int d = 1; d < TG; d *= 2) {
+            const v4f Ap = shfl_up4(A, d * LPR), Bp = shfl_up4(Bc, d * LPR);
+            if (tg >= d) {
+                Bc = A * Bp + Bc;
+                A *= Ap;
+            }
+        }
+        v4f (&buf)[MAX_WAVES][2][LPR] = agg[k & 1];
+        if (tg == TG - 1) {
+            buf[w][0][cg] = A;
+            buf[w][1][cg] = Bc;
+        }
+        const v4f Ae = shfl_up4(A, LPR), Be = shfl_up4(Bc, LPR);
+        lds_barrier();
+        if (a.saved && threadIdx.x < LPR) store_state(a.saved + (b * tiles + k) * a.C + c, carry, n);
+        v4f h = carry;
+        for (int i = 0; i < nw; ++i) {
+            if (i == w) h = carry;
+            carry = buf[i][0][cg] * carry + buf[i][1][cg];
+        }
+        if (tg > 0) h = Ae * h + Be;
+#pragma unroll
+        for (int s = 0; s < RUN; ++s) {
+            h = ag[s] * h + bv[s];
+            if (a.y && n > 0 && t + s < hi) {
+                if (a.period == 1) {
+                    store_quad<T, VEC>(y + (long)(t + s) * a.y_st, h, n);
+                } else {
+                    int r = f.r + s, q = f.q;
+                    while (r >= a.period) { r -= a.period; ++q; }
+                    if (r == a.period - 1) store_quad<T, VEC>(y + (long)q * a.y_st, h, n);
+                }
+            }
+        }
+        t = tn;
+        f.jump(dq, dr);
+    }
+    if (a.h_last && threadIdx.x < LPR) store_state(a.h_last + crow, carry, n);
+}
+
+template <typename T, int LPR, bool VEC>
+__global__ __launch_bounds__(512) void gated_scan_bwd_kernel(const HpmnGatedScanBwd a) {
+    constexpr int TG = 64 / LPR;
+    __shared__ v4f agg[2][MAX_WAVES][3][LPR];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    const int cg = lane % LPR, tg = lane / LPR;
+    const int ncb = (a.C + 4 * LPR - 1) / (4 * LPR);
+    const long b = blockIdx.x / ncb;
+    const int c = ((int)(blockIdx.x % ncb) * LPR + cg) * 4;
+    const int n = max(0, min(4, a.C - c));
+    const int step = nw * TG * RUN;
+    const int tiles = (a.T + TILE - 1) / TILE;
+    const int lo = n > 0 ? (a.begin ? a.begin[b] : 0) : a.T, hi = a.T;
+    const T *z = (const T *)a.z + b * a.z_sb + c, *v = (const T *)a.v + b * a.v_sb + c;
+    const T *dy = (const T *)a.d_y + b * a.dy_sb + c;
+    T *dz = (T *)a.d_z + b * a.dz_sb + c, *dv = (T *)a.d_v + b * a.dv_sb + c;
+    const long crow = b * a.C + c;
+
+    v4f R = {0.f, 0.f, 0.f, 0.f};            // dL/dh behind the tile
+    if (a.d_h_last) R = load_state(a.d_h_last + crow, n);
+    const int k_last = (a.T - 1) / step;
+    int t = k_last * step + (w * TG + tg) * RUN;
+    Firing f;
+    f.start(t, a.period);
+    const int dq = step / a.period, dr = step % a.period;
+    quad_t<T> zr[RUN], vr[RUN], dr_[RUN];
+    auto load_dy = [&](int at, int q0, int r0) {
+#pragma unroll
+        for (int s = 0; s < RUN; ++s) {
+            dr_[s] = quad_t<T>{};
+            if (!a.d_y || n == 0 || at + s < 0 || at + s >= hi) continue;
+            if (a.period == 1) {
+                dr_[s] = load_quad<T, VEC>(dy + (long)(at + s) * a.dy_st, n);
+            } else {
+                int r = r0 + s, q = q0;
+                while (r >= a.period) { r -= a.period; ++q; }
+                if (r == a.period - 1) dr_[s] = load_quad<T, VEC>(dy + (long)q * a.dy_st, n);
+            }
+        }
+    };
+    load_run<T, VEC>(zr, z, a.z_st, t, lo, hi, n);
+    load_run<T, VEC>(vr, v, a.v_st, t, lo, hi, n);
+    load_dy(t, f.q, f.r);
+    v4f hs = load_state(a.saved + (b * tiles + k_last) * a.C + c, n);
+    for (int k = k_last; k >= 0; --k) {
+        v4f ag[RUN], ug[RUN], vv[RUN], dd[RUN];
+        gate_run<T>(zr, t, lo, hi, ag, ug);
+#pragma unroll
+        for (int s = 0; s < RUN; ++s) {
+            vv[s] = __builtin_convertvector(vr[s], v4f);
+            dd[s] = __builtin_convertvector(dr_[s], v4f);
+        }
+        const v4f h_tile = hs;
+        const int tn = t - step;
+        f.jump(-dq, -dr);
+        if (k > 0) {
+            load_run<T, VEC>(zr, z, a.z_st, tn, lo, hi, n);
+            load_run<T, VEC>(vr, v, a.v_st, tn, lo, hi, n);
+            load_dy(tn, f.q, f.r);
+            hs = load_state(a.saved + (b * tiles + k - 1) * a.C + c, n);
+        }
+        v4f A = ag[0], Bf = ug[0] * vv[0], Br = ag[RUN - 1] * dd[RUN - 1];
+#pragma unroll
+        for (int s = 1; s < RUN; ++s) {
+            A *= ag[s];
+            Bf = ag[s] * Bf + ug[s] * vv[s];
+            Br = ag[RUN - 1 - s] * (Br + dd[RUN - 1 - s]);
+        }
+        v4f Af = A, Ar = A;                  // scanned from the front, from the back
+#pragma unroll
+        for (int d = 1; d < TG; d *= 2) {
+            const v4f Ap = shfl_up4(Af, d * LPR), Bp = shfl_up4(Bf, d * LPR);
+            const v4f An = shfl_down4(Ar, d * LPR), Bn = shfl_down4(Br, d * LPR);
+            if (tg >= d) {
+                Bf = Af * Bp + Bf;
+                Af *= Ap;
+            }
+            if (tg + d < TG) {
+                Br = Ar * Bn + Br;
+                Ar *= An;
+            }
+        }
+        v4f (&buf)[MAX_WAVES][3][LPR] = agg[k & 1];
+        if (tg == TG - 1) {
+            buf[w][0][cg] = Af;
+            buf[w][1][cg] = Bf;
+        }
+        if (tg == 0) buf[w][2][cg] = Br;
+        const v4f Ae = shfl_up4(Af, LPR), Be = shfl_up4(Bf, LPR);
+        const v4f Ax = shfl_down4(Ar, LPR), Bx = shfl_down4(Br, LPR);
+        lds_barrier();
+        v4f h = h_tile, G = R;
+        for (int i = 0; i < w; ++i) h = buf[i][0][cg] * h + buf[i][1][cg];
+        for (int i = nw - 1; i >= 0; --i) {
+            if (i == w) G = R;
+            R = buf[i][0][cg] * R + buf[i][2][cg];
+        }
+        if (tg > 0) h = Ae * h + Be;
+        if (tg < TG - 1) G = Ax * G + Bx;
+        v4f hp[RUN];
+#pragma unroll
+        for (int s = 0; s < RUN; ++s) {
+            hp[s] = h;
+            h = ag[s] * h + ug[s] * vv[s];
+        }
+#pragma unroll
+        for (int s = RUN - 1; s >= 0; --s) {
+            G += dd[s];
+            const v4f gv = ug[s] * G;
+            if (n > 0 && t + s < hi) {
+                store_quad<T, VEC>(dv + (long)(t + s) * a.dv_st, gv, n);
+                store_quad<T, VEC>(dz + (long)(t + s) * a.dz_st, gv * ag[s] * (hp[s] - vv[s]), n);
+            }
+            G = ag[s] * G;
+        }
+        t = tn;
+    }
+    if (a.d_h0 && threadIdx.x < LPR) store_state(a.d_h0 + crow, R, n);
 }
 
 __device__ __forceinline__ long step_user(const HpmnGatedStep &a, int b) {
@@ -111,19 +331,60 @@ __global__ __launch_bounds__(64) void gated_step_kernel(const HpmnGatedStep a) {
 
 size_t gated_scan_workspace_bytes(int, int, int) { return 0; }
 
+// Channels per workgroup: 64 (16 lanes per step); narrower layers take 32 or 16 channels and put more steps side by side.
+inline int scan_lanes(int C) { return C > 32 ? 16 : C > 16 ? 8 : 4; }
+// Waves: a tile of 128 steps, or as many as the whole sequence needs.
+inline int scan_waves(int T, int lpr) {
+    const int per_wave = 64 / lpr * RUN;
+    return std::min(TILE / per_wave, (T + per_wave - 1) / per_wave);
+}
+
+template <typename T>
+inline bool quads(const void *p, int64_t s0, int64_t s1) { return is_aligned(p, 4 * sizeof(T)) && s0 % 4 == 0 && s1 % 4 == 0; }
+
+template <typename T, int LPR>
+static void scan_fwd_go(const HpmnGatedScan &a, hipStream_t st) {
+    const dim3 grid((unsigned)((long)a.B * ((a.C + 4 * LPR - 1) / (4 * LPR)))), block(64 * scan_waves(a.T, LPR));
+    const bool vec = a.C % 4 == 0 && quads<T>(a.z, a.z_sb, a.z_st) && quads<T>(a.v, a.v_sb, a.v_st) && quads<T>(a.y, a.y_sb, a.y_st);
+    if (vec) hipLaunchKernelGGL((gated_scan_fwd_kernel<T, LPR, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((gated_scan_fwd_kernel<T, LPR, false>), grid, block, 0, st, a);
+}
+
+template <typename T, int LPR>
+static void scan_bwd_go(const HpmnGatedScanBwd &a, hipStream_t st) {
+    const dim3 grid((unsigned)((long)a.B * ((a.C + 4 * LPR - 1) / (4 * LPR)))), block(64 * scan_waves(a.T, LPR));
+    const bool vec = a.C % 4 == 0 && quads<T>(a.z, a.z_sb, a.z_st) && quads<T>(a.v, a.v_sb, a.v_st) && quads<T>(a.d_y, a.dy_sb, a.dy_st) &&
+                     quads<T>(a.d_z, a.dz_sb, a.dz_st) && quads<T>(a.d_v, a.dv_sb, a.dv_st);
+    if (vec) hipLaunchKernelGGL((gated_scan_bwd_kernel<T, LPR, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((gated_scan_bwd_kernel<T, LPR, false>), grid, block, 0, st, a);
+}
+
+template <typename T>
+static void scan_fwd_type(const HpmnGatedScan &a, hipStream_t st) {
+    const int lpr = scan_lanes(a.C);
+    if (lpr == 16) scan_fwd_go<T, 16>(a, st);
+    else if (lpr == 8) scan_fwd_go<T, 8>(a, st);
+    else scan_fwd_go<T, 4>(a, st);
+}
+template <typename T>
+static void scan_bwd_type(const HpmnGatedScanBwd &a, hipStream_t st) {
+    const int lpr = scan_lanes(a.C);
+    if (lpr == 16) scan_bwd_go<T, 16>(a, st);
+    else if (lpr == 8) scan_bwd_go<T, 8>(a, st);
+    else scan_bwd_go<T, 4>(a, st);
+}
+
 int gated_scan_fwd_launch(const HpmnGatedScan &a, hipStream_t st) {
-    const dim3 grid((unsigned)((long)a.B * ((a.C + 63) / 64)));
-    if (a.dtype == HPMN_F32) hipLaunchKernelGGL(gated_scan_fwd_kernel<float>, grid, dim3(64), 0, st, a);
-    else if (a.dtype == HPMN_BF16) hipLaunchKernelGGL(gated_scan_fwd_kernel<bf16_t>, grid, dim3(64), 0, st, a);
-    else hipLaunchKernelGGL(gated_scan_fwd_kernel<f16_t>, grid, dim3(64), 0, st, a);
+    if (a.dtype == HPMN_F32) scan_fwd_type<float>(a, st);
+    else if (a.dtype == HPMN_BF16) scan_fwd_type<bf16_t>(a, st);
+    else scan_fwd_type<f16_t>(a, st);
     return check_launch();
 }
 
 int gated_scan_bwd_launch(const HpmnGatedScanBwd &a, hipStream_t st) {
-    const dim3 grid((unsigned)((long)a.B * ((a.C + 63) / 64)));
-    if (a.dtype == HPMN_F32) hipLaunchKernelGGL(gated_scan_bwd_kernel<float>, grid, dim3(64), 0, st, a);
-    else if (a.dtype == HPMN_BF16) hipLaunchKernelGGL(gated_scan_bwd_kernel<bf16_t>, grid, dim3(64), 0, st, a);
-    else hipLaunchKernelGGL(gated_scan_bwd_kernel<f16_t>, grid, dim3(64), 0, st, a);
+    if (a.dtype == HPMN_F32) scan_bwd_type<float>(a, st);
+    else if (a.dtype == HPMN_BF16) scan_bwd_type<bf16_t>(a, st);
+    else scan_bwd_type<f16_t>(a, st);
     return check_launch();
 }
 
