@@ -1579,9 +1579,9 @@ _SEQ_DTYPES = {torch.float32: _lib.HPMN_F32, torch.bfloat16: _lib.HPMN_BF16, tor
 
 def _chk_seq(name, t, shape, dtype, device):
     """A device tensor of the given shape / dtype whose last dimension is dense (the others may be strided)."""
-    if not (t.is_cuda and t.device == device and t.dtype == dtype and tuple(t.shape) == tuple(shape)):
+    if t.dtype is not dtype or t.device != device or t.shape != shape:
         raise ValueError("%s: expected %s %s on %s, got %s %s on %s" % (name, tuple(shape), dtype, device, tuple(t.shape), t.dtype, t.device))
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError("%s: the last dimension has to be dense, got strides %s" % (name, t.stride()))
 
 
@@ -1599,21 +1599,26 @@ def _seq_input(name, t, ndim):
     return _SEQ_DTYPES[t.dtype]
 
 
+# (the raw handle in 0.1 us where building a Stream object takes 2: these calls are a few us in all)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call_on(device, name, fn, a):
     """fn(&a, stream) on the device's current stream, with that device current (a launch needs both to agree)."""
     if device.index == torch.cuda.current_device():
-        rc = fn(C.byref(a), torch.cuda.current_stream(device).cuda_stream)
+        rc = fn(C.byref(a), _raw_stream(device.index))
     else:
         with torch.cuda.device(device):
-            rc = fn(C.byref(a), torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, name)
+            rc = fn(C.byref(a), _raw_stream(device.index))
+    if rc != 0:
+        _lib.check(rc, name)
 
 
 def _gated_scan_shape(z, v, begin, period):
     _seq_input("z", z, 3)
     B, T, Cc = z.shape
-    _chk_seq("z", z, (B, T, Cc), z.dtype, z.device)
-    _chk_seq("v", v, (B, T, Cc), z.dtype, z.device)
+    _chk_seq("z", z, z.shape, z.dtype, z.device)
+    _chk_seq("v", v, z.shape, z.dtype, z.device)
     if begin is not None:
         if not (begin.device == z.device and begin.dtype == torch.int32 and tuple(begin.shape) == (B,) and begin.is_contiguous()):
             raise ValueError("begin: expected contiguous int32 [%d] on %s, got %s %s" % (B, z.device, begin.dtype, tuple(begin.shape)))
@@ -1653,15 +1658,10 @@ def gated_scan_fwd(z, v, *, h0=None, begin=None, period=1, train=False):
         else:
             h_last.copy_(h0)
         return y, h_last, saved
-    a = _lib.HpmnGatedScan()
-    a.B, a.T, a.C, a.dtype, a.period = B, T, Cc, _SEQ_DTYPES[z.dtype], period
-    a.z, a.v = z.data_ptr(), v.data_ptr()
-    a.z_sb, a.z_st, a.v_sb, a.v_st = z.stride(0), z.stride(1), v.stride(0), v.stride(1)
-    a.begin, a.h0 = _ptr(begin), _ptr(h0)
-    a.h0_sb = 0 if h0 is None else h0.stride(0)
-    a.y, a.y_sb, a.y_st, a.h_last, a.saved = y.data_ptr(), y.stride(0), y.stride(1), h_last.data_ptr(), _ptr(saved)
-    ws, a.workspace_bytes = _gated_scan_workspace(B, T, Cc, dev)
-    a.workspace = _ptr(ws)
+    ws, n = _gated_scan_workspace(B, T, Cc, dev)
+    a = _lib.HpmnGatedScan(B, T, Cc, _SEQ_DTYPES[z.dtype], period, 0, z.data_ptr(), v.data_ptr(), z.stride(0), z.stride(1), v.stride(0),
+                           v.stride(1), _ptr(begin), _ptr(h0), 0 if h0 is None else h0.stride(0), y.data_ptr(), T // period * Cc, Cc,
+                           h_last.data_ptr(), _ptr(saved), _ptr(ws), n)
     _call_on(dev, "hpmn_gated_scan_fwd", _lib.load().hpmn_gated_scan_fwd, a)
     return y, h_last, saved
 
@@ -1700,17 +1700,12 @@ def gated_scan_bwd(z, v, saved, d_y, *, d_h_last=None, begin=None, period=1, out
         else:
             d_h0.copy_(d_h_last)
         return d_z, d_v, d_h0
-    a = _lib.HpmnGatedScanBwd()
-    a.B, a.T, a.C, a.dtype, a.period = B, T, Cc, _SEQ_DTYPES[z.dtype], period
-    a.z, a.v = z.data_ptr(), v.data_ptr()
-    a.z_sb, a.z_st, a.v_sb, a.v_st = z.stride(0), z.stride(1), v.stride(0), v.stride(1)
-    a.begin, a.saved, a.d_h_last = _ptr(begin), saved.data_ptr(), _ptr(d_h_last)
-    if d_y is not None:
-        a.d_y, a.dy_sb, a.dy_st = d_y.data_ptr(), d_y.stride(0), d_y.stride(1)
-    a.d_z, a.d_v, a.d_h0 = d_z.data_ptr(), d_v.data_ptr(), d_h0.data_ptr()
-    a.dz_sb, a.dz_st, a.dv_sb, a.dv_st = d_z.stride(0), d_z.stride(1), d_v.stride(0), d_v.stride(1)
-    ws, a.workspace_bytes = _gated_scan_workspace(B, T, Cc, dev)
-    a.workspace = _ptr(ws)
+    ws, n = _gated_scan_workspace(B, T, Cc, dev)
+    dy_sb, dy_st = (0, 0) if d_y is None else (d_y.stride(0), d_y.stride(1))
+    a = _lib.HpmnGatedScanBwd(B, T, Cc, _SEQ_DTYPES[z.dtype], period, 0, z.data_ptr(), v.data_ptr(), z.stride(0), z.stride(1),
+                              v.stride(0), v.stride(1), _ptr(begin), saved.data_ptr(), _ptr(d_y), dy_sb, dy_st, _ptr(d_h_last),
+                              d_z.data_ptr(), d_v.data_ptr(), d_z.stride(0), d_z.stride(1), d_v.stride(0), d_v.stride(1),
+                              d_h0.data_ptr(), _ptr(ws), n)
     _call_on(dev, "hpmn_gated_scan_bwd", _lib.load().hpmn_gated_scan_bwd, a)
     return d_z, d_v, d_h0
 
@@ -1726,8 +1721,8 @@ def gated_scan_step(z, v, state, user=None, *, commit=True):
     _seq_input("z", z, 2)
     B, Cc = z.shape
     dev = z.device
-    _chk_seq("z", z, (B, Cc), z.dtype, dev)
-    _chk_seq("v", v, (B, Cc), z.dtype, dev)
+    _chk_seq("z", z, z.shape, z.dtype, dev)
+    _chk_seq("v", v, z.shape, z.dtype, dev)
     if state.dim() != 2:
         raise ValueError("state: expected [n_users, %d], got %s" % (Cc, tuple(state.shape)))
     _chk_seq("state", state, (state.shape[0], Cc), torch.float32, dev)
@@ -1740,19 +1735,32 @@ def gated_scan_step(z, v, state, user=None, *, commit=True):
     y = torch.empty(B, Cc, device=dev, dtype=z.dtype)
     if y.numel() == 0:
         return y
-    a = _lib.HpmnGatedStep()
-    a.C, a.dtype = Cc, _SEQ_DTYPES[z.dtype]
-    a.z_s, a.v_s, a.y_s = z.stride(0), v.stride(0), y.stride(0)
-    a.state, a.state_s, a.n_users = state.data_ptr(), max(state.stride(0), Cc), state.shape[0]
-    a.flags = (_lib.HPMN_STEP_COMMIT if commit else 0) | (_lib.HPMN_STEP_USER_I64 if user is not None and user.dtype == torch.int64 else 0)
+    flags = (_lib.HPMN_STEP_COMMIT if commit else 0) | (_lib.HPMN_STEP_USER_I64 if user is not None and user.dtype is torch.int64 else 0)
+    zs, vs = z.stride(0), v.stride(0)
+    a = _lib.HpmnGatedStep(B, Cc, _SEQ_DTYPES[z.dtype], flags, z.data_ptr(), v.data_ptr(), zs, vs, state.data_ptr(),
+                           max(state.stride(0), Cc), state.shape[0], _ptr(user), y.data_ptr(), Cc)
+    fn = _lib.load().hpmn_gated_scan_step
     # the ordered form works through its user list in calls of HPMN_STEP_MAX_INDEXED rows (one stream: still in row order)
-    step = _lib.HPMN_STEP_MAX_INDEXED if commit and user is not None else B
-    for lo in range(0, B, step):
-        a.B = min(step, B - lo)
-        a.z, a.v, a.y = z[lo:].data_ptr(), v[lo:].data_ptr(), y[lo:].data_ptr()
-        a.user = None if user is None else user[lo:].data_ptr()
-        _call_on(dev, "hpmn_gated_scan_step", _lib.load().hpmn_gated_scan_step, a)
+    most = _lib.HPMN_STEP_MAX_INDEXED
+    if not (commit and user is not None and B > most):
+        _call_on(dev, "hpmn_gated_scan_step", fn, a)
+        return y
+    size, wide = z.element_size(), user.element_size()
+    for lo in range(0, B, most):
+        a.B = min(most, B - lo)
+        _call_on(dev, "hpmn_gated_scan_step", fn, a)
+        a.z, a.v, a.y, a.user = a.z + most * zs * size, a.v + most * vs * size, a.y + most * Cc * size, a.user + most * wide
     return y
+
+
+def _as_rows(t, Cc):
+    """(tensor, row stride) of t as rows of Cc dense elements; what cannot be viewed that way (a permuted tensor) is copied."""
+    if t.is_contiguous():
+        return t, Cc
+    t = t.reshape(-1, Cc)
+    if Cc > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0)
 
 
 def _dropout(name, x, keep_prob, seed, offset, residual, rng):
@@ -1770,15 +1778,11 @@ def _dropout(name, x, keep_prob, seed, offset, residual, rng):
     if y.numel() == 0:
         return y
     Cc = shape[-1]
-    # 2-D views: rows at one stride.  What cannot be viewed that way (a permuted tensor) is copied into order first.
-    rows = [None if t is None else t.reshape(-1, Cc) for t in (x, residual)]
-    rows = [t if t is None or Cc == 1 or t.stride(1) == 1 else t.contiguous() for t in rows]
-    a = _lib.HpmnDropout()
-    a.N, a.C, a.dtype, a.keep_prob = y.numel() // Cc, Cc, _SEQ_DTYPES[x.dtype], keep_prob
-    a.x, a.x_s, a.y, a.y_s = rows[0].data_ptr(), rows[0].stride(0), y.data_ptr(), Cc
+    x, x_s = _as_rows(x, Cc)
     if residual is not None:
-        a.residual, a.r_s = rows[1].data_ptr(), rows[1].stride(0)
-    a.seed, a.offset, a.rng = seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _ptr(rng)
+        residual, r_s = _as_rows(residual, Cc)
+    a = _lib.HpmnDropout(y.numel() // Cc, Cc, _SEQ_DTYPES[x.dtype], keep_prob, x.data_ptr(), _ptr(residual), y.data_ptr(), x_s,
+                         0 if residual is None else r_s, Cc, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _ptr(rng))
     _call_on(dev, "hpmn_dropout", _lib.load().hpmn_dropout, a)
     return y
 
@@ -1840,16 +1844,11 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k_suffix=None, v_suffix=None,
     out = torch.empty(B, Lq, Hq, D, device=dev, dtype=q.dtype)
     lse = torch.empty(B, Lq, Hq, device=dev, dtype=torch.float32) if want_lse else None
     if out.numel() > 0:
-        a = _lib.HpmnPrefixAttn()
-        a.B, a.Lq, a.Hq, a.Hkv, a.D, a.dtype, a.P, a.S, a.scale = B, Lq, Hq, Hkv, D, dt, P, S, scale
-        a.q, a.q_sb, a.q_sl, a.q_sh = q.data_ptr(), q.stride(0), q.stride(1), q.stride(2)
-        a.k_pre, a.kp_st, a.kp_sh = k_prefix.data_ptr(), k_prefix.stride(0), k_prefix.stride(1)
-        a.v_pre, a.vp_st, a.vp_sh = v_prefix.data_ptr(), v_prefix.stride(0), v_prefix.stride(1)
-        if S:
-            a.k_suf, a.ks_sb, a.ks_st, a.ks_sh = (k_suffix.data_ptr(),) + k_suffix.stride()[:3]
-            a.v_suf, a.vs_sb, a.vs_st, a.vs_sh = (v_suffix.data_ptr(),) + v_suffix.stride()[:3]
-        a.prefix_len, a.suffix_len = _ptr(prefix_len), _ptr(suffix_len)
-        a.out, a.o_sb, a.o_sl, a.o_sh, a.lse = out.data_ptr(), out.stride(0), out.stride(1), out.stride(2), _ptr(lse)
+        ks = (k_suffix.data_ptr(), v_suffix.data_ptr()) if S else (None, None)
+        kst, vst = (k_suffix.stride()[:3], v_suffix.stride()[:3]) if S else ((0, 0, 0), (0, 0, 0))
+        a = _lib.HpmnPrefixAttn(B, Lq, Hq, Hkv, D, dt, P, S, scale, 0, q.data_ptr(), *q.stride()[:3], k_prefix.data_ptr(),
+                                v_prefix.data_ptr(), *k_prefix.stride()[:2], *v_prefix.stride()[:2], *ks, *kst, *vst, _ptr(prefix_len),
+                                _ptr(suffix_len), out.data_ptr(), Lq * Hq * D, Hq * D, D, _ptr(lse), None, 0)
         lib = _lib.load()
         a.workspace_bytes = lib.hpmn_prefix_attn_workspace_bytes(C.byref(a))
         # per call: the caching allocator keeps it on the call's stream, and a captured graph owns its own
