@@ -49,42 +49,75 @@ __device__ __forceinline__ void store_state(float *p, v4f x, int n) {
         if (i < n) p[i] = x[i];
 }
 
-// Which steps fire (t + 1 a multiple of the period), and the row they fire into, kept without a division per step.
+// Which steps fire (t + 1 a multiple of the period) and the row they fire into, kept without a division per step: q = t / period,
+// r = t % period of the step at hand.
 struct Firing {
-    int q, r, period;
-    __device__ __forceinline__ void start(int t, int p) { period = p; q = t / p; r = t - q * p; }
-    __device__ __forceinline__ void jump(int dq, int dr) {                  // by dq * period + dr steps, |dr| < period
+    int q, r;
+    __device__ __forceinline__ bool next(int period) {                      // does this step fire?  then on to the next
+        const bool fire = r == period - 1;
+        q += fire ? 1 : 0;
+        r = fire ? 0 : r + 1;
+        return fire;
+    }
+    __device__ __forceinline__ void jump(int dq, int dr, int period) {      // by dq * period + dr steps, |dr| < period
         q += dq;
         r += dr;
         if (r >= period) { r -= period; ++q; }
-        else if (r < 0) { r += period; --q; }
+        if (r < 0) { r += period; --q; }
     }
 };
 
-// z, v: dense channels at row strides; one lane's run of RUN steps from step t on, only steps in [lo, hi) are touched.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_run(quad_t<T> (&q)[RUN], const T *p, long stride, int t, int lo, int hi, int n) {
-#pragma unroll
-    for (int s = 0; s < RUN; ++s) {
-        q[s] = quad_t<T>{};
-        if (t + s >= lo && t + s < hi) q[s] = load_quad<T, VEC>(p + (long)(t + s) * stride, n);
-    }
+// Row `row` of a [T, ...] operand: row strides fit 32 bits (checked by the entry point), so the offset is ONE 32 x 32 -> 64 bit
+// multiply-add; a 64-bit stride takes three, at a quarter of the rate.
+template <typename T>
+__device__ __forceinline__ T *at_row(T *p, unsigned row, int64_t stride) {
+    return p + (uint64_t)row * (uint32_t)stride;
 }
 
-// a and u of a run; steps outside [lo, hi) are the identity (a = 1, u = 0, whatever was or was not loaded).
+// A lane's share of the work: its channels [c, c + n) (n = 0: none, it repeats another lane's loads and stores nothing), and the
+// steps [lo, hi) that count.  Loads always go to a row in [lo, hi) (to one valid row if there is none), so that none is conditional.
+struct Share {
+    int c, n, nl, lo, hi;
+    __device__ __forceinline__ Share(int C, int T, int first, int begin) {
+        n = max(0, min(4, C - first));
+        c = n > 0 ? first : max(0, C - 4);
+        nl = n > 0 ? n : min(4, C);
+        lo = max(0, begin);
+        hi = T;
+    }
+    __device__ __forceinline__ unsigned row(int t) const { return (unsigned)min(max(t, min(lo, hi - 1)), hi - 1); }
+    __device__ __forceinline__ bool live(int t) const { return t >= lo && t < hi; }
+};
+
+// a, u and v of a run.  Steps that do not count are the identity (a = 1, u = 0, v = 0) whatever was loaded for them.
 template <typename T>
-__device__ __forceinline__ void gate_run(const quad_t<T> (&zr)[RUN], int t, int lo, int hi, v4f (&ag)[RUN], v4f (&ug)[RUN]) {
+__device__ __forceinline__ void gate_run(const Share &sh, bool whole, int t, const quad_t<T> (&zr)[RUN], const quad_t<T> (&vr)[RUN],
+                                         v4f (&ag)[RUN], v4f (&ug)[RUN], v4f (&vv)[RUN]) {
 #pragma unroll
     for (int s = 0; s < RUN; ++s) {
-        const bool live = t + s >= lo && t + s < hi;
+        ag[s] = __builtin_convertvector(zr[s], v4f);
+        vv[s] = __builtin_convertvector(vr[s], v4f);
+    }
+    if (!whole) {
+#pragma unroll
+        for (int s = 0; s < RUN; ++s) {
+            const bool live = sh.live(t + s);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                ag[s][i] = live ? ag[s][i] : 1e30f;          // sigmoid: exactly 1, and its complement 0
+                vv[s][i] = live ? vv[s][i] : 0.f;
+            }
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < RUN; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float x, y;
-            gate_pair((float)zr[s][i], x, y);
-            ag[s][i] = live ? x : 1.f;
-            ug[s][i] = live ? y : 0.f;
+            gate_pair(ag[s][i], x, y);
+            ag[s][i] = x;
+            ug[s][i] = y;
         }
-    }
 }
 
 template <typename T, int LPR, bool VEC>
@@ -95,35 +128,32 @@ __global__ __launch_bounds__(512) void gated_scan_fwd_kernel(const HpmnGatedScan
     const int cg = lane % LPR, tg = lane / LPR;
     const int ncb = (a.C + 4 * LPR - 1) / (4 * LPR);
     const long b = blockIdx.x / ncb;
-    const int c = ((int)(blockIdx.x % ncb) * LPR + cg) * 4;
-    const int n = max(0, min(4, a.C - c));   // this lane's channels (0: none, it only takes part in the exchange)
+    const Share sh(a.C, a.T, ((int)(blockIdx.x % ncb) * LPR + cg) * 4, a.begin ? a.begin[b] : 0);
     const int step = nw * TG * RUN;          // steps per tile (TILE, or fewer when the whole sequence fits)
-    const int tiles = (a.T + TILE - 1) / TILE;
-    const int lo = n > 0 ? (a.begin ? a.begin[b] : 0) : a.T, hi = a.T;
-    const T *z = (const T *)a.z + b * a.z_sb + c, *v = (const T *)a.v + b * a.v_sb + c;
-    T *y = (T *)a.y + b * a.y_sb + c;
-    const long crow = b * a.C + c;
+    const int tiles = (a.T + TILE - 1) / TILE, period = a.period;
+    const T *z = (const T *)a.z + b * a.z_sb + sh.c, *v = (const T *)a.v + b * a.v_sb + sh.c;
+    T *y = (T *)a.y + b * a.y_sb + sh.c;
 
     v4f carry = {0.f, 0.f, 0.f, 0.f};
-    if (a.h0) carry = load_state(a.h0 + b * a.h0_sb + c, n);
+    if (a.h0) carry = load_state(a.h0 + b * a.h0_sb + sh.c, sh.n);
     int t = (w * TG + tg) * RUN;
-    Firing f;
-    f.start(t, a.period);
-    const int dq = step / a.period, dr = step % a.period;
+    Firing f = {t / period, t % period};
+    const int dq = step / period, dr = step % period;
     quad_t<T> zr[RUN], vr[RUN];
-    load_run<T, VEC>(zr, z, a.z_st, t, lo, hi, n);
-    load_run<T, VEC>(vr, v, a.v_st, t, lo, hi, n);
-    for (int k = 0, t0 = 0; t0 < a.T; ++k, t0 += step) {
-        v4f ag[RUN], bv[RUN];
-        gate_run<T>(zr, t, lo, hi, ag, bv);
+    auto load = [&](int at) {
 #pragma unroll
         for (int s = 0; s < RUN; ++s) {
-            // (steps outside were not loaded: their v is zero)
-            bv[s] *= __builtin_convertvector(vr[s], v4f);
+            zr[s] = load_quad<T, VEC>(at_row(z, sh.row(at + s), a.z_st), sh.nl);
+            vr[s] = load_quad<T, VEC>(at_row(v, sh.row(at + s), a.v_st), sh.nl);
         }
-        const int tn = t + step;
-        load_run<T, VEC>(zr, z, a.z_st, tn, lo, hi, n);
-        load_run<T, VEC>(vr, v, a.v_st, tn, lo, hi, n);
+    };
+    load(t);
+    for (int k = 0, t0 = 0; t0 < a.T; ++k, t0 += step) {
+        v4f ag[RUN], bv[RUN], vv[RUN];
+        gate_run<T>(sh, t0 >= sh.lo && t0 + step <= sh.hi, t, zr, vr, ag, bv, vv);
+#pragma unroll
+        for (int s = 0; s < RUN; ++s) bv[s] *= vv[s];
+        load(t + step);
         v4f A = ag[0], Bc = bv[0];
 #pragma unroll
         for (int s = 1; s < RUN; ++s) {
@@ -145,30 +175,24 @@ __global__ __launch_bounds__(512) void gated_scan_fwd_kernel(const HpmnGatedScan
         }
         const v4f Ae = shfl_up4(A, LPR), Be = shfl_up4(Bc, LPR);
         lds_barrier();
-        if (a.saved && threadIdx.x < LPR) store_state(a.saved + (b * tiles + k) * a.C + c, carry, n);
+        if (a.saved && threadIdx.x < LPR) store_state(a.saved + (b * tiles + k) * a.C + sh.c, carry, sh.n);
         v4f h = carry;
         for (int i = 0; i < nw; ++i) {
             if (i == w) h = carry;
             carry = buf[i][0][cg] * carry + buf[i][1][cg];
         }
         if (tg > 0) h = Ae * h + Be;
+        Firing g = f;
 #pragma unroll
         for (int s = 0; s < RUN; ++s) {
             h = ag[s] * h + bv[s];
-            if (a.y && n > 0 && t + s < hi) {
-                if (a.period == 1) {
-                    store_quad<T, VEC>(y + (long)(t + s) * a.y_st, h, n);
-                } else {
-                    int r = f.r + s, q = f.q;
-                    while (r >= a.period) { r -= a.period; ++q; }
-                    if (r == a.period - 1) store_quad<T, VEC>(y + (long)q * a.y_st, h, n);
-                }
-            }
+            const unsigned row = (unsigned)g.q;
+            if (g.next(period) && a.y && sh.n > 0 && t + s < sh.hi) store_quad<T, VEC>(at_row(y, row, a.y_st), h, sh.n);
         }
-        t = tn;
-        f.jump(dq, dr);
+        t += step;
+        f.jump(dq, dr, period);
     }
-    if (a.h_last && threadIdx.x < LPR) store_state(a.h_last + crow, carry, n);
+    if (a.h_last && threadIdx.x < LPR) store_state(a.h_last + b * a.C + sh.c, carry, sh.n);
 }
 
 template <typename T, int LPR, bool VEC>
@@ -179,59 +203,56 @@ __global__ __launch_bounds__(512) void gated_scan_bwd_kernel(const HpmnGatedScan
     const int cg = lane % LPR, tg = lane / LPR;
     const int ncb = (a.C + 4 * LPR - 1) / (4 * LPR);
     const long b = blockIdx.x / ncb;
-    const int c = ((int)(blockIdx.x % ncb) * LPR + cg) * 4;
-    const int n = max(0, min(4, a.C - c));
+    const Share sh(a.C, a.T, ((int)(blockIdx.x % ncb) * LPR + cg) * 4, a.begin ? a.begin[b] : 0);
     const int step = nw * TG * RUN;
-    const int tiles = (a.T + TILE - 1) / TILE;
-    const int lo = n > 0 ? (a.begin ? a.begin[b] : 0) : a.T, hi = a.T;
-    const T *z = (const T *)a.z + b * a.z_sb + c, *v = (const T *)a.v + b * a.v_sb + c;
-    const T *dy = (const T *)a.d_y + b * a.dy_sb + c;
-    T *dz = (T *)a.d_z + b * a.dz_sb + c, *dv = (T *)a.d_v + b * a.dv_sb + c;
-    const long crow = b * a.C + c;
+    const int tiles = (a.T + TILE - 1) / TILE, period = a.period;
+    const T *z = (const T *)a.z + b * a.z_sb + sh.c, *v = (const T *)a.v + b * a.v_sb + sh.c;
+    // (without d_y its loads go to z, which has at least as many rows, and are not used)
+    const bool has_dy = a.d_y != nullptr;
+    const T *dy = has_dy ? (const T *)a.d_y + b * a.dy_sb + sh.c : z;
+    const long dy_st = has_dy ? a.dy_st : a.z_st;
+    const int dy_rows = a.T / period;
+    T *dz = (T *)a.d_z + b * a.dz_sb + sh.c, *dv = (T *)a.d_v + b * a.dv_sb + sh.c;
 
     v4f R = {0.f, 0.f, 0.f, 0.f};            // dL/dh behind the tile
-    if (a.d_h_last) R = load_state(a.d_h_last + crow, n);
+    if (a.d_h_last) R = load_state(a.d_h_last + b * a.C + sh.c, sh.n);
     const int k_last = (a.T - 1) / step;
     int t = k_last * step + (w * TG + tg) * RUN;
-    Firing f;
-    f.start(t, a.period);
-    const int dq = step / a.period, dr = step % a.period;
-    quad_t<T> zr[RUN], vr[RUN], dr_[RUN];
-    auto load_dy = [&](int at, int q0, int r0) {
+    Firing f = {t / period, t % period};
+    const int dq = step / period, dr = step % period;
+    quad_t<T> zr[RUN], vr[RUN], yr[RUN];
+    v4f hs;
+    auto load = [&](int at, int k, Firing g) {
 #pragma unroll
         for (int s = 0; s < RUN; ++s) {
-            dr_[s] = quad_t<T>{};
-            if (!a.d_y || n == 0 || at + s < 0 || at + s >= hi) continue;
-            if (a.period == 1) {
-                dr_[s] = load_quad<T, VEC>(dy + (long)(at + s) * a.dy_st, n);
-            } else {
-                int r = r0 + s, q = q0;
-                while (r >= a.period) { r -= a.period; ++q; }
-                if (r == a.period - 1) dr_[s] = load_quad<T, VEC>(dy + (long)q * a.dy_st, n);
+            zr[s] = load_quad<T, VEC>(at_row(z, sh.row(at + s), a.z_st), sh.nl);
+            vr[s] = load_quad<T, VEC>(at_row(v, sh.row(at + s), a.v_st), sh.nl);
+            yr[s] = load_quad<T, VEC>(at_row(dy, (unsigned)max(0, min(g.q, dy_rows - 1)), dy_st), sh.nl);
+            g.next(period);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) hs[i] = a.saved[(b * tiles + max(k, 0)) * a.C + sh.c + min(i, sh.nl - 1)];
+    };
+    load(t, k_last, f);
+    for (int k = k_last; k >= 0; --k) {
+        const int t0 = k * step;
+        v4f ag[RUN], ug[RUN], vv[RUN], dd[RUN];
+        const bool whole = t0 >= sh.lo && t0 + step <= sh.hi;
+        gate_run<T>(sh, whole, t, zr, vr, ag, ug, vv);
+#pragma unroll
+        for (int s = 0; s < RUN; ++s) dd[s] = __builtin_convertvector(yr[s], v4f);
+        if (!(has_dy && period == 1 && t0 + step <= sh.hi)) {
+            Firing g = f;
+#pragma unroll
+            for (int s = 0; s < RUN; ++s) {
+                const bool fire = g.next(period) && has_dy && t + s < sh.hi;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dd[s][i] = fire ? dd[s][i] : 0.f;
             }
         }
-    };
-    load_run<T, VEC>(zr, z, a.z_st, t, lo, hi, n);
-    load_run<T, VEC>(vr, v, a.v_st, t, lo, hi, n);
-    load_dy(t, f.q, f.r);
-    v4f hs = load_state(a.saved + (b * tiles + k_last) * a.C + c, n);
-    for (int k = k_last; k >= 0; --k) {
-        v4f ag[RUN], ug[RUN], vv[RUN], dd[RUN];
-        gate_run<T>(zr, t, lo, hi, ag, ug);
-#pragma unroll
-        for (int s = 0; s < RUN; ++s) {
-            vv[s] = __builtin_convertvector(vr[s], v4f);
-            dd[s] = __builtin_convertvector(dr_[s], v4f);
-        }
         const v4f h_tile = hs;
-        const int tn = t - step;
-        f.jump(-dq, -dr);
-        if (k > 0) {
-            load_run<T, VEC>(zr, z, a.z_st, tn, lo, hi, n);
-            load_run<T, VEC>(vr, v, a.v_st, tn, lo, hi, n);
-            load_dy(tn, f.q, f.r);
-            hs = load_state(a.saved + (b * tiles + k - 1) * a.C + c, n);
-        }
+        f.jump(-dq, -dr, period);
+        load(t - step, k - 1, f);
         v4f A = ag[0], Bf = ug[0] * vv[0], Br = ag[RUN - 1] * dd[RUN - 1];
 #pragma unroll
         for (int s = 1; s < RUN; ++s) {
@@ -280,15 +301,15 @@ __global__ __launch_bounds__(512) void gated_scan_bwd_kernel(const HpmnGatedScan
         for (int s = RUN - 1; s >= 0; --s) {
             G += dd[s];
             const v4f gv = ug[s] * G;
-            if (n > 0 && t + s < hi) {
-                store_quad<T, VEC>(dv + (long)(t + s) * a.dv_st, gv, n);
-                store_quad<T, VEC>(dz + (long)(t + s) * a.dz_st, gv * ag[s] * (hp[s] - vv[s]), n);
+            if (sh.n > 0 && t + s < sh.hi) {
+                store_quad<T, VEC>(at_row(dv, (unsigned)(t + s), a.dv_st), gv, sh.n);
+                store_quad<T, VEC>(at_row(dz, (unsigned)(t + s), a.dz_st), gv * ag[s] * (hp[s] - vv[s]), sh.n);
             }
             G = ag[s] * G;
         }
-        t = tn;
+        t -= step;
     }
-    if (a.d_h0 && threadIdx.x < LPR) store_state(a.d_h0 + crow, R, n);
+    if (a.d_h0 && threadIdx.x < LPR) store_state(a.d_h0 + b * a.C + sh.c, R, sh.n);
 }
 
 __device__ __forceinline__ long step_user(const HpmnGatedStep &a, int b) {

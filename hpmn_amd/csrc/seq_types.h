@@ -16,7 +16,8 @@ template <> struct Quad<bf16_t> { typedef bf16x4 type; };
 template <> struct Quad<f16_t> { typedef f16x4 type; };
 template <typename T> using quad_t = typename Quad<T>::type;
 
-// Four elements at p (VEC: one aligned access) or the n < 4 valid ones of them (!VEC: scalar accesses, zero behind).
+// Four elements from p on (VEC: one aligned access), or the n in 1..4 valid ones of them (!VEC: scalar accesses; the rest repeat
+// the last valid one).  Unconditional in every lane: a load under a condition is waited for where the paths meet.
 template <typename T, bool VEC>
 __device__ __forceinline__ quad_t<T> load_quad(const T *p, int n) {
     if constexpr (VEC) {
@@ -24,7 +25,7 @@ __device__ __forceinline__ quad_t<T> load_quad(const T *p, int n) {
     } else {
         quad_t<T> q;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = i < n ? p[i] : (T)0.f;
+        for (int i = 0; i < 4; ++i) q[i] = p[min(i, n - 1)];
         return q;
     }
 }
@@ -39,14 +40,13 @@ __device__ __forceinline__ void store_quad(T *p, v4f x, int n) {
     }
 }
 
-// a = sigmoid(z) and u = 1 - a = sigmoid(-z), both to a relative rounding or two: e = exp(-|z|) <= 1 never overflows, and the
-// smaller of the two is e / (1 + e) instead of a difference (1 - a in fp32 has no digits left from z = 17 on).
+// a = sigmoid(z) = 1 / (1 + e) and u = 1 - a = e / (1 + e) with e = exp(-z): both to a rounding or two of THEMSELVES (1 - a as a
+// difference has no digits left from z = 17 on).  e is capped at 2^120, where a has long stopped mattering beside u = 1 (and
+// inf * 0 would be NaN); the cap is the minimum that keeps a NaN.  Six instructions, two of them on the transcendental unit.
 __device__ __forceinline__ void gate_pair(float z, float &a, float &u) {
-    const float e = __builtin_amdgcn_exp2f(NEG_LOG2E * fabsf(z));
-    const float big = __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
-    const bool pos = z >= 0.f;
-    a = pos ? big : small;
-    u = pos ? small : big;
+    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(NEG_LOG2E * z, 120.0f));
+    a = __builtin_amdgcn_rcpf(1.0f + e);
+    u = e * a;
 }
 
 inline bool is_aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }

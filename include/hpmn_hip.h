@@ -790,8 +790,8 @@ int hpmn_memory_update(const HpmnOnlineUpdate *args, void *stream);
  *
  *   a_t = sigmoid(z_t),   h_t = a_t h_{t-1} + (1 - a_t) v_t,   y_j = h_{(j+1) period - 1}      j < T / period
  *
- * z, v: [B, T, C] of `dtype`; element strides over b and t are arguments (two halves of one projection buffer), the last
- * dimension is dense.  States, gates and sums are fp32 whatever the dtype; y, d_z, d_v are rounded to it once.
+ * z, v: [B, T, C] of `dtype`; element strides over b and t (below 2^31 over t) are arguments (two halves of one projection
+ * buffer), the last dimension is dense.  States, gates and sums are fp32 whatever the dtype; y, d_z, d_v are rounded to it once.
  *   begin  : optional [B] int32: front padding.  Steps t < begin[b] are identities (h_t = h_{t-1}, whatever z and v hold
  *            there, NaN included) and have zero gradients; begin[b] >= T: nothing but padding.
  *   h0     : optional [B, C] (row stride h0_sb): the state in front of step 0; NULL: zero.
