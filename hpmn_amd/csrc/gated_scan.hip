@@ -120,23 +120,157 @@ __device__ __forceinline__ void gate_run(const Share &sh, bool whole, int t, con
         }
 }
 
-template <typename T, int LPR, bool VEC>
-__global__ __launch_bounds__(512) void gated_scan_fwd_kernel(const HpmnGatedScan a) {
-    constexpr int TG = 64 / LPR;             // runs side by side in a wave
-    __shared__ v4f agg[2][MAX_WAVES][2][LPR];
+// Few sequences, long ones: the time axis is cut into chunks of whole tiles and a first launch composes every chunk to one map
+// (A, B) per channel; the main launch then starts each chunk from the maps in front of it (behind it, in the backward).  z and v
+// are read a second time, mostly from the caches; no workgroup waits for another.
+struct ChunkArgs {
+    int T, C, period;
+    const void *z, *x;                       // x: v, or d_y in the backward
+    int64_t z_sb, z_st, x_sb, x_st;
+    const int32_t *begin;
+    float *ws;                               // [B][chunks][2][C]
+    int chunks, tiles;                       // per sequence, per chunk
+};
+
+template <typename T, int LPR, bool VEC, bool BWD>
+__global__ __launch_bounds__(512) void gated_scan_chunk_kernel(const ChunkArgs a) {
+    constexpr int TG = 64 / LPR;
+    __shared__ v4f agg[MAX_WAVES][2][LPR];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
     const int cg = lane % LPR, tg = lane / LPR;
     const int ncb = (a.C + 4 * LPR - 1) / (4 * LPR);
-    const long b = blockIdx.x / ncb;
-    const Share sh(a.C, a.T, ((int)(blockIdx.x % ncb) * LPR + cg) * 4, a.begin ? a.begin[b] : 0);
+    const int chunk = blockIdx.x % a.chunks, rest = blockIdx.x / a.chunks;
+    const long b = rest / ncb;
+    if (chunk == (BWD ? 0 : a.chunks - 1)) return;           // nobody starts behind the last (in front of the first) one
+    const Share sh(a.C, a.T, ((rest % ncb) * LPR + cg) * 4, a.begin ? a.begin[b] : 0);
+    const T *z = (const T *)a.z + b * a.z_sb + sh.c;
+    const bool has_x = a.x != nullptr;
+    const T *x = has_x ? (const T *)a.x + b * a.x_sb + sh.c : z;
+    const long x_st = has_x ? a.x_st : a.z_st;
+    const int x_rows = BWD ? a.T / a.period : a.T;
+    // a lane group owns a span of a.tiles * RUN consecutive steps here, so that its map is composed without an exchange
+    const int span = a.tiles * RUN, t_first = chunk * a.tiles * TILE + (w * TG + tg) * span;
+    v4f A = {1.f, 1.f, 1.f, 1.f}, Bc = {0.f, 0.f, 0.f, 0.f};
+    quad_t<T> zr[RUN], xr[RUN];
+    auto load = [&](int j) {
+        const int t = t_first + (BWD ? span - RUN - j : j);
+        Firing g = {t / a.period, t % a.period};
+#pragma unroll
+        for (int s = 0; s < RUN; ++s) {
+            zr[s] = load_quad<T, VEC>(at_row(z, sh.row(t + s), a.z_st), sh.nl);
+            const unsigned row = BWD ? (unsigned)max(0, min(g.q, x_rows - 1)) : sh.row(t + s);
+            xr[s] = load_quad<T, VEC>(at_row(x, row, x_st), sh.nl);
+            g.next(a.period);
+        }
+    };
+    load(0);
+    for (int j = 0; j < span; j += RUN) {
+        const int t = t_first + (BWD ? span - RUN - j : j);
+        v4f ag[RUN], ug[RUN], vv[RUN];
+        gate_run<T>(sh, false, t, zr, xr, ag, ug, vv);
+        if (BWD) {
+            Firing g = {t / a.period, t % a.period};
+#pragma unroll
+            for (int s = 0; s < RUN; ++s) {
+                const bool fire = g.next(a.period) && has_x && t + s < sh.hi;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vv[s][i] = fire ? (float)xr[s][i] : 0.f;
+            }
+        }
+        load(min(j + RUN, span - RUN));
+#pragma unroll
+        for (int s = 0; s < RUN; ++s) {
+            if (BWD) {
+                Bc = ag[RUN - 1 - s] * (Bc + vv[RUN - 1 - s]);
+                A *= ag[RUN - 1 - s];
+            } else {
+                Bc = ag[s] * Bc + ug[s] * vv[s];
+                A *= ag[s];
+            }
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < TG; d *= 2) {                        // neighbours in pairs: the earlier map first (the later, in the backward)
+        const v4f Ao = BWD ? shfl_down4(A, d * LPR) : shfl_up4(A, d * LPR), Bo = BWD ? shfl_down4(Bc, d * LPR) : shfl_up4(Bc, d * LPR);
+        if (BWD ? tg + d < TG : tg >= d) {
+            Bc = A * Bo + Bc;
+            A *= Ao;
+        }
+    }
+    if (tg == (BWD ? 0 : TG - 1)) {
+        agg[w][0][cg] = A;
+        agg[w][1][cg] = Bc;
+    }
+    __syncthreads();
+    if (threadIdx.x >= LPR) return;
+    A = v4f{1.f, 1.f, 1.f, 1.f};
+    Bc = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < nw; ++i) {
+        const int j = BWD ? nw - 1 - i : i;
+        Bc = agg[j][0][cg] * Bc + agg[j][1][cg];
+        A *= agg[j][0][cg];
+    }
+    float *out = a.ws + (b * a.chunks + chunk) * 2 * a.C + sh.c;
+    store_state(out, A, sh.n);
+    store_state(out + a.C, Bc, sh.n);
+}
+
+// The state behind chunks first, first + dir, ... (count <= TILE of them) when it is `start` in front: the chunk maps go through the
+// same lanes / shuffles / LDS composition as the steps of a tile.
+template <int LPR>
+__device__ __forceinline__ v4f fold_chunks(const float *ws, int C, int c, int nl, int first, int dir, int count, v4f start,
+                                           v4f (&buf)[MAX_WAVES][2][LPR]) {
+    constexpr int TG = 64 / LPR;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6, cg = lane % LPR, tg = lane / LPR;
+    v4f A = {1.f, 1.f, 1.f, 1.f}, Bc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < RUN; ++s) {
+        const int p = (w * TG + tg) * RUN + s;
+        if (p >= count) continue;
+        const float *m = ws + (long)(first + dir * p) * 2 * C + c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = m[min(i, nl - 1)];
+            Bc[i] = x * Bc[i] + m[C + min(i, nl - 1)];
+            A[i] *= x;
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < TG; d *= 2) {
+        const v4f Ap = shfl_up4(A, d * LPR), Bp = shfl_up4(Bc, d * LPR);
+        if (tg >= d) {
+            Bc = A * Bp + Bc;
+            A *= Ap;
+        }
+    }
+    if (tg == TG - 1) {
+        buf[w][0][cg] = A;
+        buf[w][1][cg] = Bc;
+    }
+    lds_barrier();
+    for (int i = 0; i < nw; ++i) start = buf[i][0][cg] * start + buf[i][1][cg];
+    return start;
+}
+
+template <typename T, int LPR, bool VEC>
+__global__ __launch_bounds__(512) void gated_scan_fwd_kernel(const HpmnGatedScan a, int chunks, int chunk_tiles) {
+    constexpr int TG = 64 / LPR;             // runs side by side in a wave
+    __shared__ v4f agg[2][MAX_WAVES][2][LPR], maps[MAX_WAVES][2][LPR];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    const int cg = lane % LPR, tg = lane / LPR;
+    const int ncb = (a.C + 4 * LPR - 1) / (4 * LPR);
+    const int chunk = blockIdx.x % chunks, rest = blockIdx.x / chunks;
+    const long b = rest / ncb;
+    const Share sh(a.C, a.T, ((rest % ncb) * LPR + cg) * 4, a.begin ? a.begin[b] : 0);
     const int step = nw * TG * RUN;          // steps per tile (TILE, or fewer when the whole sequence fits)
+    const int k_first = chunk * chunk_tiles, t_end = min(a.T, (k_first + chunk_tiles) * step);
     const int tiles = (a.T + TILE - 1) / TILE, period = a.period;
     const T *z = (const T *)a.z + b * a.z_sb + sh.c, *v = (const T *)a.v + b * a.v_sb + sh.c;
     T *y = (T *)a.y + b * a.y_sb + sh.c;
 
     v4f carry = {0.f, 0.f, 0.f, 0.f};
     if (a.h0) carry = load_state(a.h0 + b * a.h0_sb + sh.c, sh.n);
-    int t = (w * TG + tg) * RUN;
+    int t = k_first * step + (w * TG + tg) * RUN;
     Firing f = {t / period, t % period};
     const int dq = step / period, dr = step % period;
     quad_t<T> zr[RUN], vr[RUN];
@@ -148,7 +282,9 @@ __global__ __launch_bounds__(512) void gated_scan_fwd_kernel(const HpmnGatedScan
         }
     };
     load(t);
-    for (int k = 0, t0 = 0; t0 < a.T; ++k, t0 += step) {
+    if (chunk > 0)
+        carry = fold_chunks<LPR>((const float *)a.workspace + b * chunks * 2 * a.C, a.C, sh.c, sh.nl, 0, 1, chunk, carry, maps);
+    for (int k = k_first, t0 = k_first * step; t0 < t_end; ++k, t0 += step) {
         v4f ag[RUN], bv[RUN], vv[RUN];
         gate_run<T>(sh, t0 >= sh.lo && t0 + step <= sh.hi, t, zr, vr, ag, bv, vv);
 #pragma unroll
@@ -192,18 +328,19 @@ __global__ __launch_bounds__(512) void gated_scan_fwd_kernel(const HpmnGatedScan
         t += step;
         f.jump(dq, dr, period);
     }
-    if (a.h_last && threadIdx.x < LPR) store_state(a.h_last + b * a.C + sh.c, carry, sh.n);
+    if (a.h_last && chunk == chunks - 1 && threadIdx.x < LPR) store_state(a.h_last + b * a.C + sh.c, carry, sh.n);
 }
 
 template <typename T, int LPR, bool VEC>
-__global__ __launch_bounds__(512) void gated_scan_bwd_kernel(const HpmnGatedScanBwd a) {
+__global__ __launch_bounds__(512) void gated_scan_bwd_kernel(const HpmnGatedScanBwd a, int chunks, int chunk_tiles) {
     constexpr int TG = 64 / LPR;
-    __shared__ v4f agg[2][MAX_WAVES][3][LPR];
+    __shared__ v4f agg[2][MAX_WAVES][3][LPR], maps[MAX_WAVES][2][LPR];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
     const int cg = lane % LPR, tg = lane / LPR;
     const int ncb = (a.C + 4 * LPR - 1) / (4 * LPR);
-    const long b = blockIdx.x / ncb;
-    const Share sh(a.C, a.T, ((int)(blockIdx.x % ncb) * LPR + cg) * 4, a.begin ? a.begin[b] : 0);
+    const int chunk = blockIdx.x % chunks, rest = blockIdx.x / chunks;
+    const long b = rest / ncb;
+    const Share sh(a.C, a.T, ((rest % ncb) * LPR + cg) * 4, a.begin ? a.begin[b] : 0);
     const int step = nw * TG * RUN;
     const int tiles = (a.T + TILE - 1) / TILE, period = a.period;
     const T *z = (const T *)a.z + b * a.z_sb + sh.c, *v = (const T *)a.v + b * a.v_sb + sh.c;
@@ -216,7 +353,7 @@ __global__ __launch_bounds__(512) void gated_scan_bwd_kernel(const HpmnGatedScan
 
     v4f R = {0.f, 0.f, 0.f, 0.f};            // dL/dh behind the tile
     if (a.d_h_last) R = load_state(a.d_h_last + b * a.C + sh.c, sh.n);
-    const int k_last = (a.T - 1) / step;
+    const int k_first = chunk * chunk_tiles, k_last = min((a.T - 1) / step, k_first + chunk_tiles - 1);
     int t = k_last * step + (w * TG + tg) * RUN;
     Firing f = {t / period, t % period};
     const int dq = step / period, dr = step % period;
@@ -234,7 +371,10 @@ __global__ __launch_bounds__(512) void gated_scan_bwd_kernel(const HpmnGatedScan
         for (int i = 0; i < 4; ++i) hs[i] = a.saved[(b * tiles + max(k, 0)) * a.C + sh.c + min(i, sh.nl - 1)];
     };
     load(t, k_last, f);
-    for (int k = k_last; k >= 0; --k) {
+    if (chunk < chunks - 1)
+        R = fold_chunks<LPR>((const float *)a.workspace + b * chunks * 2 * a.C, a.C, sh.c, sh.nl, chunks - 1, -1, chunks - 1 - chunk, R,
+                             maps);
+    for (int k = k_last; k >= k_first; --k) {
         const int t0 = k * step;
         v4f ag[RUN], ug[RUN], vv[RUN], dd[RUN];
         const bool whole = t0 >= sh.lo && t0 + step <= sh.hi;
@@ -309,7 +449,7 @@ __global__ __launch_bounds__(512) void gated_scan_bwd_kernel(const HpmnGatedScan
         }
         t -= step;
     }
-    if (a.d_h0 && threadIdx.x < LPR) store_state(a.d_h0 + b * a.C + sh.c, R, sh.n);
+    if (a.d_h0 && chunk == 0 && threadIdx.x < LPR) store_state(a.d_h0 + b * a.C + sh.c, R, sh.n);
 }
 
 __device__ __forceinline__ long step_user(const HpmnGatedStep &a, int b) {
@@ -350,8 +490,6 @@ __global__ __launch_bounds__(64) void gated_step_kernel(const HpmnGatedStep a) {
     }
 }
 
-size_t gated_scan_workspace_bytes(int, int, int) { return 0; }
-
 // Channels per workgroup: 64 (16 lanes per step); narrower layers take 32 or 16 channels and put more steps side by side.
 inline int scan_lanes(int C) { return C > 32 ? 16 : C > 16 ? 8 : 4; }
 // Waves: a tile of 128 steps, or as many as the whole sequence needs.
@@ -360,24 +498,59 @@ inline int scan_waves(int T, int lpr) {
     return std::min(TILE / per_wave, (T + per_wave - 1) / per_wave);
 }
 
+struct Cut {
+    int chunks, tiles;                       // per sequence, per chunk
+};
+// Time chunks where whole sequences leave two thirds of the CUs idle and there are at least four tiles to share out: as many as
+// fill the CUs once (twice costs more than it hides: the backward has the registers for one workgroup per CU), at most TILE of
+// them (fold_chunks).  Forward / backward us, cut against whole, fp32, C = 64, device time:
+//   8 x 1024: 11 / 14 against 19 / 28;   64 x 4096: 55 / 80 against 65 / 130;   1 x 16384: 14 / 17 against 241 / 379;
+//   at the rule's borders: 64 x 512 12.4 / 17.1 against 11.7 / 17.6, 80 x 1024 19 / 27 against 20 / 31;
+//   beyond them: 96 x 1024 (two chunks) 26 / 33 against 21 / 32, 8 x 256 (two tiles) 10 / 12 against 7 / 10.
+static Cut scan_cut(int B, int T, int C) {
+    const int lpr = scan_lanes(C), tiles = (T + TILE - 1) / TILE;
+    const long whole = (long)B * ((C + 4 * lpr - 1) / (4 * lpr));
+    const int want = (int)std::min<long>(std::min(tiles, TILE), 256 / whole);
+    if (want < 3 || tiles < 4) return {1, tiles};
+    const int per = (tiles + want - 1) / want;
+    return {(tiles + per - 1) / per, per};
+}
+
+size_t gated_scan_workspace_bytes(int B, int T, int C) {
+    const Cut cut = scan_cut(B, T, C);
+    return cut.chunks > 1 ? (size_t)B * cut.chunks * 2 * C * sizeof(float) : 0;
+}
+
 template <typename T>
 inline bool quads(const void *p, int64_t s0, int64_t s1) { return is_aligned(p, 4 * sizeof(T)) && s0 % 4 == 0 && s1 % 4 == 0; }
 
 template <typename T, int LPR>
 static void scan_fwd_go(const HpmnGatedScan &a, hipStream_t st) {
-    const dim3 grid((unsigned)((long)a.B * ((a.C + 4 * LPR - 1) / (4 * LPR)))), block(64 * scan_waves(a.T, LPR));
+    const Cut cut = scan_cut(a.B, a.T, a.C);
+    const dim3 grid((unsigned)((long)a.B * ((a.C + 4 * LPR - 1) / (4 * LPR)) * cut.chunks)), block(64 * scan_waves(a.T, LPR));
     const bool vec = a.C % 4 == 0 && quads<T>(a.z, a.z_sb, a.z_st) && quads<T>(a.v, a.v_sb, a.v_st) && quads<T>(a.y, a.y_sb, a.y_st);
-    if (vec) hipLaunchKernelGGL((gated_scan_fwd_kernel<T, LPR, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((gated_scan_fwd_kernel<T, LPR, false>), grid, block, 0, st, a);
+    if (cut.chunks > 1) {
+        const ChunkArgs c = {a.T, a.C, 1, a.z, a.v, a.z_sb, a.z_st, a.v_sb, a.v_st, a.begin, (float *)a.workspace, cut.chunks, cut.tiles};
+        if (vec) hipLaunchKernelGGL((gated_scan_chunk_kernel<T, LPR, true, false>), grid, block, 0, st, c);
+        else hipLaunchKernelGGL((gated_scan_chunk_kernel<T, LPR, false, false>), grid, block, 0, st, c);
+    }
+    if (vec) hipLaunchKernelGGL((gated_scan_fwd_kernel<T, LPR, true>), grid, block, 0, st, a, cut.chunks, cut.tiles);
+    else hipLaunchKernelGGL((gated_scan_fwd_kernel<T, LPR, false>), grid, block, 0, st, a, cut.chunks, cut.tiles);
 }
 
 template <typename T, int LPR>
 static void scan_bwd_go(const HpmnGatedScanBwd &a, hipStream_t st) {
-    const dim3 grid((unsigned)((long)a.B * ((a.C + 4 * LPR - 1) / (4 * LPR)))), block(64 * scan_waves(a.T, LPR));
+    const Cut cut = scan_cut(a.B, a.T, a.C);
+    const dim3 grid((unsigned)((long)a.B * ((a.C + 4 * LPR - 1) / (4 * LPR)) * cut.chunks)), block(64 * scan_waves(a.T, LPR));
     const bool vec = a.C % 4 == 0 && quads<T>(a.z, a.z_sb, a.z_st) && quads<T>(a.v, a.v_sb, a.v_st) && quads<T>(a.d_y, a.dy_sb, a.dy_st) &&
                      quads<T>(a.d_z, a.dz_sb, a.dz_st) && quads<T>(a.d_v, a.dv_sb, a.dv_st);
-    if (vec) hipLaunchKernelGGL((gated_scan_bwd_kernel<T, LPR, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((gated_scan_bwd_kernel<T, LPR, false>), grid, block, 0, st, a);
+    if (cut.chunks > 1) {
+        const ChunkArgs c = {a.T, a.C, a.period, a.z, a.d_y, a.z_sb, a.z_st, a.dy_sb, a.dy_st, a.begin, (float *)a.workspace, cut.chunks, cut.tiles};
+        if (vec) hipLaunchKernelGGL((gated_scan_chunk_kernel<T, LPR, true, true>), grid, block, 0, st, c);
+        else hipLaunchKernelGGL((gated_scan_chunk_kernel<T, LPR, false, true>), grid, block, 0, st, c);
+    }
+    if (vec) hipLaunchKernelGGL((gated_scan_bwd_kernel<T, LPR, true>), grid, block, 0, st, a, cut.chunks, cut.tiles);
+    else hipLaunchKernelGGL((gated_scan_bwd_kernel<T, LPR, false>), grid, block, 0, st, a, cut.chunks, cut.tiles);
 }
 
 template <typename T>
