@@ -104,7 +104,7 @@ int hpmn_dropout(const HpmnDropout *a, void *stream) {
     if (!aligned_to(a->x, a->dtype) || !aligned_to(a->y, a->dtype) || !aligned_to(a->residual, a->dtype)) return HPMN_EINVAL;
     if (!is_aligned(a->rng, 8)) return HPMN_EINVAL;
     if (a->x_s < 0 || a->r_s < 0 || (a->N > 1 && a->y_s < a->C)) return HPMN_EINVAL;
-    if (a->N > (1l << 40) / a->C) return HPMN_EUNSUPPORTED;      // one launch: blocks of 2048 elements in a 31-bit grid
+    if (a->N > (1l << 40) / a->C) return HPMN_EUNSUPPORTED;      // one launch: 2^30 blocks of at least 1024 elements
     // floor(p 2^16 + 1/2), as a double: p is a float, so the product is exact
     const double q = (double)a->keep_prob * 65536.0 + 0.5;
     const unsigned thr = q < 1.0 ? 1u : (unsigned)q;
