@@ -37,7 +37,7 @@ BASE_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"]
 # Sources compiled WITHOUT the packed fp32 instructions (v_pk_add / mul / fma_f32): the compiler forms them out of ordinary float
 # code, their use is not audited form by form in these kernels, and none of them is bound by the fp32 rate.  The GRU scans keep
 # them: their serial mat-vecs are written for packed FMAs (without: C3 2.45 -> 2.74 ms per step).
-NO_PACKED_FP32 = ("gated_scan.hip", "seq_api.hip", "dropout.hip", "prefix_attn.hip")
+NO_PACKED_FP32 = ("gated_scan.hip", "seq_api.hip", "dropout.hip", "prefix_attn.hip", "prefix_attn_bf16.hip", "prefix_attn_f16.hip")
 NO_PACKED_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 

@@ -1,0 +1,467 @@
+// Attention of a batch that shares a long prefix: the kernel, a template over the element type (one translation unit per type
+// instantiates it: prefix_attn.hip, prefix_attn_bf16.hip, prefix_attn_f16.hip).
+//
+// The query rows of one key head -- every (sequence, query token, grouped head) -- are a matrix of M = B Lq Hq / Hkv rows against the
+// SAME prefix, so the prefix is a matrix product's operand: a workgroup takes 128 rows (or 32, when there are few) and a range of
+// keys, and K and V are read once per 128 rows instead of once per row.  One pass with the running maximum and sum:
+//   S^T = K Q^T   a wave: 32 query rows (columns of S^T: one row per lane pair, so maximum and sum are a register reduction and ONE
+//                 exchange between the wave's halves), 32 keys at a time on the matrix pipe, Q in registers throughout;
+//   O^T += V^T P  P is used where it lies: S^T's accumulator layout is the operand layout of the second product up to an order of
+//                 the keys, and V is read in that order (16-bit: transposing LDS reads, four keys x 16 columns per 16 lanes).
+// K and V tiles go global -> registers -> LDS, the next tile in flight while this one is used; LDS chunks of 16 bytes are permuted
+// by the row number so that neither the reads along a row nor those across eight rows meet in a bank.
+// Few rows: the four waves of a workgroup share out the keys of a tile instead of the rows and join their results in LDS.  The key
+// axis is split over workgroups until the chip is full; a second kernel joins the parts (maximum, sum, unnormalised output in fp32).
+// A row's own suffix is the same thing with M = Lq Hq / Hkv rows and a key limit per row, in the same launch.
+//
+// Rounding choices: scores, maxima, sums and outputs are fp32; the probabilities are rounded to the 16-bit type once, as operand of
+// the second product (half a step each, independent, so about one more rounding of the result).  fp16 probabilities are scaled by
+// 2^15: unscaled, everything below 2^-24 of the largest would vanish, which for long prefixes is most of them.
+#pragma once
+#include <algorithm>
+#include <cfloat>
+#include <type_traits>
+
+#include "seq_types.h"
+
+namespace hpmn {
+
+struct AttnPlan {
+    int mw_pre, mw_suf;                      // waves along the rows (the other 4 / mw along the keys)
+    int rt_pre, rt_suf;                      // row tiles per key head / per sequence and key head
+    int splits_pre, splits_suf, per_pre, per_suf;   // key ranges and their length
+    int parts;                               // splits_pre + splits_suf; 1: no second kernel, results go straight out
+    int d4;                                  // D rounded up to 4: a row of a part
+    long rows;                               // Hkv * M
+    long o_at;                               // where the parts' outputs start in the workspace, in floats (behind their m and l)
+    unsigned blocks_pre, blocks_suf;
+};
+
+AttnPlan attn_plan(const HpmnPrefixAttn &a);
+template <typename T> int prefix_attn_type(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st);
+
+// Keys per tile and LDS bytes of a configuration.
+constexpr int attn_sub(int esize, int mw) { return esize == 2 && mw == 4 ? 2 : 1; }
+constexpr int attn_tile(int esize, int mw) { return 4 / mw * 32 * attn_sub(esize, mw); }
+constexpr size_t attn_lds(int esize, int dp, int mw) {
+    const size_t tiles = (size_t)2 * attn_tile(esize, mw) * dp * esize, join = (size_t)4 * 32 * (dp + 4) * 4 + 4 * 32 * 8;
+    return mw == 4 ? tiles : std::max(tiles, join);
+}
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef float v8f __attribute__((ext_vector_type(8)));
+
+template <typename T> struct Frag;
+template <> struct Frag<bf16_t> {
+    typedef bf16x8 type;
+    static __device__ __forceinline__ v16f mma(bf16x8 a, bf16x8 b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Frag<f16_t> {
+    typedef f16x8 type;
+    static __device__ __forceinline__ v16f mma(f16x8 a, f16x8 b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Frag<float> { typedef v4f type; };
+
+constexpr float LN2 = 0.69314718055994530942f;
+
+// barrier that orders LDS alone: __syncthreads() would wait for the tile in flight
+__device__ __forceinline__ void attn_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Position of 16-byte chunk c of row `row`: eight neighbouring rows put a chunk into eight different bank groups, four neighbouring
+// rows a pair of chunks into four.
+template <int CPR>
+__device__ __forceinline__ int chunk_at(int row, int c) {
+    const int f = CPR >= 8 ? ((row & 3) << 1) | ((row >> 2) & 1) : (row & 2) | ((row >> 2) & 1);
+    return row * CPR + (c ^ f);
+}
+
+struct AttnKeys {
+    const void *K, *V;                       // key head's (and sequence's) first row
+    int64_t kst, vst;
+    int begin, end;                          // this workgroup's keys, inside the length
+    int part;
+    bool suffix;
+    int b, seen;                             // suffix: its sequence, and suffix_len - Lq + 1: query token i sees seen + i keys
+};
+
+template <typename T, int DP, bool VEC, int MW>
+__device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &p, char *lds, const AttnKeys &src, int kvh, int row0,
+                                       int row_end) {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int KW = 4 / MW, SUB = attn_sub(sizeof(T), MW), KT = attn_tile(sizeof(T), MW);
+    constexpr int EPC = 16 / sizeof(T), CPR = DP / EPC, LD = KT * CPR / 256, DT = DP / 32;
+    constexpr float OFF = std::is_same<T, f16_t>::value ? 15.f : 0.f;
+    constexpr float LAZY = OFF > 0.f ? 0.f : 8.f;       // the maximum may lag by 2^LAZY before O is rescaled
+    typedef typename Frag<T>::type frag;
+    char *Kt = lds, *Vt = lds + KT * DP * (int)sizeof(T);
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, n = lane & 31;
+    const int mw = w % MW, kw = w / MW;
+    const int group = a.Hq / a.Hkv, per_seq = a.Lq * group;
+    const int row = row0 + mw * 32 + n;
+    const bool active = row0 + mw * 32 < row_end;       // (wave-uniform)
+    const int r = min(row, row_end - 1);
+    const int in_seq = src.suffix ? r : r % per_seq, b = src.suffix ? src.b : r / per_seq;
+    const int tok = in_seq / group, h = kvh * group + in_seq % group;
+    const int limit = src.suffix ? min(src.end, max(0, src.seen + tok)) : src.end;
+
+    // Q: column `row` of the first product's second operand, d in the order of the chunks this half of the wave reads
+    frag qf[DP / (2 * EPC)];
+    {
+        const T *q = (const T *)a.q + b * a.q_sb + tok * a.q_sl + h * a.q_sh;
+#pragma unroll
+        for (int s = 0; s < DP / (2 * EPC); ++s) {
+            const int d0 = (2 * s + half) * EPC;
+            if constexpr (VEC) {
+                const frag x = *(const frag *)(q + (d0 < a.D ? d0 : 0));
+#pragma unroll
+                for (int e = 0; e < EPC; ++e) qf[s][e] = d0 < a.D ? x[e] : (T)0.f;
+            } else {
+#pragma unroll
+                for (int e = 0; e < EPC; ++e) {
+                    const T x = q[min(d0 + e, a.D - 1)];
+                    qf[s][e] = d0 + e < a.D ? x : (T)0.f;
+                }
+            }
+        }
+        // a negative scale becomes a sign of q, a zero one a zero q: what multiplies the scores is positive
+        if (a.scale <= 0.f) {
+#pragma unroll
+            for (int s = 0; s < DP / (2 * EPC); ++s)
+#pragma unroll
+                for (int e = 0; e < EPC; ++e) qf[s][e] = a.scale < 0.f ? -qf[s][e] : (T)0.f;
+        }
+    }
+    const float c = a.scale == 0.f ? 1.f : -NEG_LOG2E * fabsf(a.scale);
+
+    // this thread's chunks of a tile: one column of chunks, rows 256 / CPR apart
+    const int lc = tid % CPR, lrow = tid / CPR;
+    u32x4 kr[LD], vr[LD];
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int key = min(k0 + lrow + i * (256 / CPR), src.end - 1);
+            const T *k = (const T *)src.K + key * src.kst, *v = (const T *)src.V + key * src.vst;
+            if constexpr (VEC) {
+                const int d = lc * EPC < a.D ? lc * EPC : 0;
+                kr[i] = *(const u32x4 *)(k + d);
+                vr[i] = *(const u32x4 *)(v + d);
+            } else {
+                union { T e[EPC]; u32x4 u; } x, y;
+#pragma unroll
+                for (int e = 0; e < EPC; ++e) {
+                    const int d = lc * EPC + e;
+                    const T ke = k[min(d, a.D - 1)], ve = v[min(d, a.D - 1)];
+                    x.e[e] = d < a.D ? ke : (T)0.f;
+                    y.e[e] = d < a.D ? ve : (T)0.f;
+                }
+                kr[i] = x.u;
+                vr[i] = y.u;
+            }
+        }
+    };
+    auto stage = [&](int k0) {
+        const bool whole = k0 + KT <= src.end && DP == a.D;
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int lr = lrow + i * (256 / CPR);
+            u32x4 k = kr[i], v = vr[i];
+            if (!whole && (k0 + lr >= src.end || (VEC && lc * EPC >= a.D))) {   // (zeros, not what lies there: 0 * NaN)
+                k = u32x4{0, 0, 0, 0};
+                v = u32x4{0, 0, 0, 0};
+            }
+            *(u32x4 *)(Kt + 16 * chunk_at<CPR>(lr, lc)) = k;
+            *(u32x4 *)(Vt + 16 * chunk_at<CPR>(lr, lc)) = v;
+        }
+    };
+
+    v16f o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+    float m = -FLT_MAX, l = 0.f;
+
+    if (src.begin < src.end) fetch(src.begin);
+    for (int k0 = src.begin; k0 < src.end; k0 += KT) {
+        attn_barrier();                                  // the last tile has been read
+        stage(k0);
+        attn_barrier();
+        if (k0 + KT < src.end) fetch(k0 + KT);
+        const int kb = kw * 32 * SUB;
+        if (!active || k0 + kb >= src.end) continue;
+        v16f s[SUB];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+#pragma unroll
+            for (int x = 0; x < DP / (2 * EPC); ++x) {
+                const frag kf = *(const frag *)(Kt + 16 * chunk_at<CPR>(kb + 32 * u + n, 2 * x + half));
+                if constexpr (F32) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], qf[x][e], s[u], 0, 0, 0);
+                } else {
+                    s[u] = Frag<T>::mma(kf, qf[x], s[u]);
+                }
+            }
+        }
+        if (src.suffix || k0 + KT > src.end) {
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (k0 + kb + 32 * u + 8 * (i / 4) + 4 * half + i % 4 >= limit) s[u][i] = -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32)) * c;
+        if (__any(mx > m + LAZY)) {
+            const float mn = fmaxf(m, mx), keep = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= keep;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] *= keep;
+        }
+        const float mo = OFF - m;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], c, mo));
+                l += s[u][i];
+            }
+            if constexpr (F32) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int vrow = kb + 32 * u + 8 * (i / 4) + 4 * half + i % 4;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) {
+                        const int d = 32 * t + n;
+                        const float v = *(const float *)(Vt + 16 * chunk_at<CPR>(vrow, d / 4) + 4 * (d % 4));
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[u][i], o[t], 0, 0, 0);
+                    }
+                }
+            } else {
+                typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+                const int l16 = lane & 15, vr0 = kb + 32 * u + 4 * half + (l16 >> 2), vc = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    v8f pf;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) pf[i] = s[u][8 * g + i];
+                    const frag pb = __builtin_convertvector(pf, frag);
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) {
+                        union { s16x4 q[2]; frag f; } x;
+                        x.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(Vt + 16 * chunk_at<CPR>(vr0 + 16 * g, 4 * t + vc) + 8 * (l16 & 1)));
+                        x.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(Vt + 16 * chunk_at<CPR>(vr0 + 16 * g + 8, 4 * t + vc) + 8 * (l16 & 1)));
+                        o[t] = Frag<T>::mma(x.f, pb, o[t]);
+                    }
+                }
+            }
+        }
+    }
+    l += __shfl_xor(l, 32);
+    m -= OFF;
+
+    // results: quads of four neighbouring d of a row
+    float *ml = (float *)a.workspace, *parts = ml + p.o_at;
+    const long M = p.rows / a.Hkv;
+    auto put_ml = [&](int rr, int bb, int tt, int hh, float mm, float ll) {
+        if (p.parts > 1) {
+            float *at = ml + (src.part * p.rows + kvh * M + (src.suffix ? (long)bb * per_seq : 0) + rr) * 2;
+            at[0] = mm;
+            at[1] = ll;
+        } else if (a.lse) {
+            a.lse[((long)bb * a.Lq + tt) * a.Hq + hh] = ll == 0.f ? -INFINITY : (mm + __builtin_amdgcn_logf(ll)) * LN2;
+        }
+    };
+    auto put_quad = [&](int rr, int bb, int tt, int hh, int d, v4f x, float ll) {
+        if (d >= a.D) return;
+        if (p.parts > 1) {
+            *(v4f *)(parts + (src.part * p.rows + kvh * M + (src.suffix ? (long)bb * per_seq : 0) + rr) * p.d4 + d) = x;
+        } else {
+            const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+            T *out = (T *)a.out + bb * a.o_sb + tt * a.o_sl + hh * a.o_sh + d;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (d + i < a.D) out[i] = (T)(x[i] * inv);
+        }
+    };
+    if constexpr (KW == 1) {
+        if (row >= row_end) return;
+        if (half == 0) put_ml(row, b, tok, h, m, l);
+        if (l == 0.f && p.parts > 1) return;             // (nothing was seen: the second kernel does not look)
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                put_quad(row, b, tok, h, 32 * t + 8 * g + 4 * half, v4f{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]}, l);
+    } else {
+        constexpr int RS = DP + 4;                       // a row of the join, in floats
+        float *ob = (float *)lds, *mb = ob + 4 * 32 * RS;
+        attn_barrier();
+        if (active) {
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *(v4f *)(ob + (w * 32 + n) * RS + 32 * t + 8 * g + 4 * half) = v4f{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]};
+            if (half == 0) {
+                mb[(w * 32 + n) * 2] = m;
+                mb[(w * 32 + n) * 2 + 1] = l;
+            }
+        }
+        attn_barrier();
+        for (int i = tid; i < MW * 32 * (DP / 4); i += 256) {
+            const int jr = i / (DP / 4), d = i % (DP / 4) * 4, rr = row0 + jr;
+            if (rr >= row_end) break;
+            float mm = -FLT_MAX, ll = 0.f;
+#pragma unroll
+            for (int k = 0; k < KW; ++k) mm = fmaxf(mm, mb[((k * MW + jr / 32) * 32 + jr % 32) * 2]);
+            v4f x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KW; ++k) {
+                const int at = (k * MW + jr / 32) * 32 + jr % 32;
+                const float f = __builtin_amdgcn_exp2f(mb[at * 2] - mm);
+                ll += f * mb[at * 2 + 1];
+                x += f * *(const v4f *)(ob + at * RS + d);
+            }
+            const int is = src.suffix ? rr : rr % per_seq, bb = src.suffix ? src.b : rr / per_seq;
+            if (d == 0) put_ml(rr, bb, is / group, kvh * group + is % group, mm, ll);
+            put_quad(rr, bb, is / group, kvh * group + is % group, d, x, ll);
+        }
+    }
+}
+
+template <typename T, int DP, bool VEC, int MWP, int MWS>
+__global__ __launch_bounds__(256, 2) void prefix_attn_kernel(const HpmnPrefixAttn a, const AttnPlan p) {
+    extern __shared__ char attn_smem[];
+    const int group = a.Hq / a.Hkv;
+    AttnKeys k;
+    if (blockIdx.x < p.blocks_pre) {
+        // the row tiles of one key range on one XCD (workgroups go round the eight): its L2 then holds the range
+        const unsigned x = blockIdx.x % 8, j = blockIdx.x / 8;
+        const int g = (int)(j / p.rt_pre * 8 + x);
+        if (g >= a.Hkv * p.splits_pre) return;
+        const int kvh = g / p.splits_pre, split = g % p.splits_pre, rt = (int)(j % p.rt_pre);
+        const int len = a.prefix_len ? min(max(*a.prefix_len, 0), a.P) : a.P;
+        k.K = (const T *)a.k_pre + kvh * a.kp_sh;
+        k.V = (const T *)a.v_pre + kvh * a.vp_sh;
+        k.kst = a.kp_st;
+        k.vst = a.vp_st;
+        k.begin = split * p.per_pre;
+        k.end = min(len, k.begin + p.per_pre);
+        k.part = split;
+        k.suffix = false;
+        k.b = k.seen = 0;
+        attend<T, DP, VEC, MWP>(a, p, attn_smem, k, kvh, rt * 32 * MWP, a.B * a.Lq * group);
+    } else {
+        unsigned j = blockIdx.x - p.blocks_pre;
+        const int rt = j % p.rt_suf;
+        j /= p.rt_suf;
+        const int split = j % p.splits_suf;
+        j /= p.splits_suf;
+        const int kvh = j % a.Hkv, b = j / a.Hkv;
+        const int len = a.suffix_len ? min(max(a.suffix_len[b], 0), a.S) : a.S;
+        k.K = (const T *)a.k_suf + b * a.ks_sb + kvh * a.ks_sh;
+        k.V = (const T *)a.v_suf + b * a.vs_sb + kvh * a.vs_sh;
+        k.kst = a.ks_st;
+        k.vst = a.vs_st;
+        k.begin = split * p.per_suf;
+        k.end = min(len, k.begin + p.per_suf);
+        k.part = p.splits_pre + split;
+        k.suffix = true;
+        k.b = b;
+        k.seen = len - a.Lq + 1;
+        attend<T, DP, VEC, MWS>(a, p, attn_smem, k, kvh, rt * 32 * MWS, a.Lq * group);
+    }
+}
+
+// Second kernel: a wave per row joins its parts.
+template <typename T>
+__global__ __launch_bounds__(256) void prefix_attn_join_kernel(const HpmnPrefixAttn a, const AttnPlan p) {
+    const long R = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (R >= p.rows) return;
+    const int lane = threadIdx.x & 63;
+    const float *ml = (const float *)a.workspace, *parts = ml + p.o_at;
+    float m = -FLT_MAX;
+    for (int k = lane; k < p.parts; k += 64)
+        if (ml[(k * p.rows + R) * 2 + 1] != 0.f) m = fmaxf(m, ml[(k * p.rows + R) * 2]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    // 32 lanes cover a row's quads (D <= 128), two parts side by side
+    const int q = lane & 31;
+    float l = 0.f;
+    v4f x = {0.f, 0.f, 0.f, 0.f};
+    for (int k = lane >> 5; k < p.parts; k += 2) {
+        const float lk = ml[(k * p.rows + R) * 2 + 1];
+        if (lk == 0.f) continue;
+        const float f = __builtin_amdgcn_exp2f(ml[(k * p.rows + R) * 2] - m);
+        l += f * lk;
+        if (4 * q < a.D) x += f * *(const v4f *)(parts + (k * p.rows + R) * p.d4 + 4 * q);
+    }
+    l += __shfl_xor(l, 32);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] += __shfl_xor(x[i], 32);
+    if (lane >= 32) return;
+    const int group = a.Hq / a.Hkv, per_seq = a.Lq * group;
+    const long M = p.rows / a.Hkv;
+    const int kvh = (int)(R / M), r = (int)(R % M), b = r / per_seq, tok = r % per_seq / group, h = kvh * group + r % group;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    T *out = (T *)a.out + b * a.o_sb + tok * a.o_sl + h * a.o_sh + 4 * q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (4 * q + i < a.D) out[i] = (T)(x[i] * inv);
+    if (a.lse && q == 0) a.lse[((long)b * a.Lq + tok) * a.Hq + h] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+template <typename T, int DP, bool VEC, int MWP, int MWS>
+static int attn_go(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
+    const size_t lds = std::max(attn_lds(sizeof(T), DP, MWP), attn_lds(sizeof(T), DP, MWS));
+    auto kernel = prefix_attn_kernel<T, DP, VEC, MWP, MWS>;
+    if (lds > 64 * 1024) {
+        hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) {
+            set_last_hip_error((int)e);
+            return HPMN_EHIP;
+        }
+    }
+    hipLaunchKernelGGL(kernel, dim3(p.blocks_pre + p.blocks_suf), dim3(256), lds, st, a, p);
+    int rc = check_launch();
+    if (rc == HPMN_OK && p.parts > 1) {
+        hipLaunchKernelGGL(prefix_attn_join_kernel<T>, dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0, st, a, p);
+        rc = check_launch();
+    }
+    return rc;
+}
+
+template <typename T, int DP, bool VEC>
+static int attn_rows(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
+    constexpr int FEW = sizeof(T) == 4 ? 2 : 1;
+    if (p.mw_pre != 4) return attn_go<T, DP, VEC, FEW, FEW>(a, p, st);
+    return p.mw_suf == 4 ? attn_go<T, DP, VEC, 4, 4>(a, p, st) : attn_go<T, DP, VEC, 4, FEW>(a, p, st);
+}
+
+template <typename T>
+int prefix_attn_type(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
+    constexpr int E = 16 / sizeof(T);
+    bool vec = a.D % E == 0;
+    for (const void *q : {a.q, a.k_pre, a.v_pre, a.k_suf, a.v_suf}) vec = vec && is_aligned(q, 16);
+    for (int64_t s : {a.q_sb, a.q_sl, a.q_sh, a.kp_st, a.kp_sh, a.vp_st, a.vp_sh, a.ks_sb, a.ks_st, a.ks_sh, a.vs_sb, a.vs_st, a.vs_sh})
+        vec = vec && s % E == 0;
+    if (a.D <= 32) return vec ? attn_rows<T, 32, true>(a, p, st) : attn_rows<T, 32, false>(a, p, st);
+    if (a.D <= 64) return vec ? attn_rows<T, 64, true>(a, p, st) : attn_rows<T, 64, false>(a, p, st);
+    return vec ? attn_rows<T, 128, true>(a, p, st) : attn_rows<T, 128, false>(a, p, st);
+}
+
+}  // namespace hpmn

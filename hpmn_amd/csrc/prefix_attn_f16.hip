@@ -1,0 +1,8 @@
+// f16 instantiation of the shared-prefix attention (prefix_attn.h).
+#include "prefix_attn.h"
+
+namespace hpmn {
+
+template int prefix_attn_type<f16_t>(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st);
+
+}  // namespace hpmn
