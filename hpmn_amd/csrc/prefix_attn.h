@@ -71,11 +71,11 @@ constexpr float LN2 = 0.69314718055994530942f;
 // barrier that orders LDS alone: __syncthreads() would wait for the tile in flight
 __device__ __forceinline__ void attn_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// Position of 16-byte chunk c of row `row`: eight neighbouring rows put a chunk into eight different bank groups, four neighbouring
-// rows a pair of chunks into four.
+// Position of 16-byte chunk c of row `row`, CPR chunks to a row: the chunk number is permuted so that one chunk of sixteen
+// neighbouring rows (K), and four chunks of four neighbouring rows (V), each cover the 64 banks once.
 template <int CPR>
 __device__ __forceinline__ int chunk_at(int row, int c) {
-    const int f = CPR >= 8 ? ((row & 3) << 1) | ((row >> 2) & 1) : (row & 2) | ((row >> 2) & 1);
+    const int f = CPR >= 16 ? ((row & 3) << 2) | ((row >> 2) & 3) : CPR == 8 ? ((row & 2) << 1) | ((row >> 2) & 3) : (row >> 2) & 3;
     return row * CPR + (c ^ f);
 }
 
@@ -387,33 +387,68 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(const HpmnPrefixAtt
     }
 }
 
-// Second kernel: a wave per row joins its parts.
-template <typename T>
+// Second kernel: joins a row's parts.  Groups of 32 lanes (a quad of the row each, D <= 128) take the parts in turn; BLOCK: a
+// workgroup of eight groups per row, else a wave of two.  The weights of the first 64 parts of a group's turn are worked out side
+// by side in the lanes first, so that the loop over the parts is loads that depend on nothing.
+template <typename T, bool BLOCK>
 __global__ __launch_bounds__(256) void prefix_attn_join_kernel(const HpmnPrefixAttn a, const AttnPlan p) {
-    const long R = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (R >= p.rows) return;
-    const int lane = threadIdx.x & 63;
+    constexpr int GROUPS = BLOCK ? 8 : 2;
+    __shared__ float top[4];
+    __shared__ v4f sums[BLOCK ? 8 : 1][32];
+    __shared__ float ls[8];
+    const long R = BLOCK ? (long)blockIdx.x : (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (R >= p.rows) return;                             // (whole waves; BLOCK: never)
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane & 31, grp = BLOCK ? (int)threadIdx.x >> 5 : lane >> 5;
     const float *ml = (const float *)a.workspace, *parts = ml + p.o_at;
     float m = -FLT_MAX;
-    for (int k = lane; k < p.parts; k += 64)
-        if (ml[(k * p.rows + R) * 2 + 1] != 0.f) m = fmaxf(m, ml[(k * p.rows + R) * 2]);
+    for (int k = BLOCK ? (int)threadIdx.x : lane; k < p.parts; k += BLOCK ? 256 : 64) {
+        const float mk = ml[(k * p.rows + R) * 2], lk = ml[(k * p.rows + R) * 2 + 1];
+        m = fmaxf(m, lk != 0.f ? mk : -FLT_MAX);
+    }
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    // 32 lanes cover a row's quads (D <= 128), two parts side by side
-    const int q = lane & 31;
+    if (BLOCK) {
+        if (lane == 0) top[w] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    }
     float l = 0.f;
     v4f x = {0.f, 0.f, 0.f, 0.f};
-    for (int k = lane >> 5; k < p.parts; k += 2) {
-        const float lk = ml[(k * p.rows + R) * 2 + 1];
-        if (lk == 0.f) continue;
-        const float f = __builtin_amdgcn_exp2f(ml[(k * p.rows + R) * 2] - m);
-        l += f * lk;
-        if (4 * q < a.D) x += f * *(const v4f *)(parts + (k * p.rows + R) * p.d4 + 4 * q);
-    }
-    l += __shfl_xor(l, 32);
+    const int d0 = min(4 * q, p.d4 - 4);
+    for (int k0 = grp; k0 < p.parts; k0 += 32 * GROUPS) {
+        const int mine = k0 + q * GROUPS;                // lane q of the group: the weight of the turn's q-th part
+        float f = 0.f;
+        if (mine < p.parts) {
+            const float lk = ml[(mine * p.rows + R) * 2 + 1];
+            f = lk != 0.f ? __builtin_amdgcn_exp2f(ml[(mine * p.rows + R) * 2] - m) : 0.f;
+            l += f * lk;
+        }
+        const int count = min(32, (p.parts - k0 + GROUPS - 1) / GROUPS);
+#pragma unroll 8
+        for (int j = 0; j < count; ++j) {
+            const float fj = __shfl(f, (lane & 32) + j);
+            const v4f o = *(const v4f *)(parts + ((long)(k0 + j * GROUPS) * p.rows + R) * p.d4 + d0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] += __shfl_xor(x[i], 32);
-    if (lane >= 32) return;
+            for (int i = 0; i < 4; ++i) x[i] += fj != 0.f ? fj * o[i] : 0.f;       // (an empty part was not written)
+        }
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor(l, d);
+    if (BLOCK) {
+        sums[grp][q] = x;
+        if (q == 0) ls[grp] = l;
+        __syncthreads();
+        if (threadIdx.x >= 32) return;
+        for (int g = 1; g < 8; ++g) {
+            x += sums[g][q];
+            l += ls[g];
+        }
+    } else {
+        l += __shfl_xor(l, 32);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] += __shfl_xor(x[i], 32);
+        if (lane >= 32) return;
+    }
     const int group = a.Hq / a.Hkv, per_seq = a.Lq * group;
     const long M = p.rows / a.Hkv;
     const int kvh = (int)(R / M), r = (int)(R % M), b = r / per_seq, tok = r % per_seq / group, h = kvh * group + r % group;
@@ -439,7 +474,9 @@ static int attn_go(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
     hipLaunchKernelGGL(kernel, dim3(p.blocks_pre + p.blocks_suf), dim3(256), lds, st, a, p);
     int rc = check_launch();
     if (rc == HPMN_OK && p.parts > 1) {
-        hipLaunchKernelGGL(prefix_attn_join_kernel<T>, dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0, st, a, p);
+        // a workgroup per row while that makes up to eight a CU or the parts are many
+        if (p.rows <= 2048 || p.parts > 32) hipLaunchKernelGGL((prefix_attn_join_kernel<T, true>), dim3((unsigned)p.rows), dim3(256), 0, st, a, p);
+        else hipLaunchKernelGGL((prefix_attn_join_kernel<T, false>), dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0, st, a, p);
         rc = check_launch();
     }
     return rc;
