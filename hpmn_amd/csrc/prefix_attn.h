@@ -33,6 +33,7 @@ struct AttnPlan {
     int parts;                               // splits_pre + splits_suf; 1: no second kernel, results go straight out
     int d4;                                  // D rounded up to 4: a row of a part
     long rows;                               // Hkv * M
+    int wide;                                // the prefix's row strides fit attend_whole_tiles (32-bit lane offsets)
     long o_at;                               // where the parts' outputs start in the workspace, in floats (behind their m and l)
     unsigned blocks_pre, blocks_suf;
 };
@@ -45,7 +46,7 @@ constexpr int attn_sub(int esize, int mw) { return esize == 2 && mw == 4 ? 2 : 1
 constexpr int attn_tile(int esize, int mw) { return 4 / mw * 32 * attn_sub(esize, mw); }
 constexpr size_t attn_lds(int esize, int dp, int mw) {
     const size_t tiles = (size_t)2 * attn_tile(esize, mw) * dp * esize, join = (size_t)4 * 32 * (dp + 4) * 4 + 4 * 32 * 8;
-    return mw == 4 ? tiles : std::max(tiles, join);
+    return mw == 4 ? (esize == 2 ? 2 * tiles : tiles) : std::max(tiles, join);
 }
 
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -79,6 +80,15 @@ __device__ __forceinline__ int chunk_at(int row, int c) {
     return row * CPR + (c ^ f);
 }
 
+// x of the lane 32 away (one VALU instruction; a shuffle goes through LDS).  The swap exchanges the upper half of its first operand
+// with the lower half of its second; the copy is opaque because with two equal operands the compiler takes the two results for one.
+__device__ __forceinline__ float other_half(float x) {
+    unsigned a = __builtin_bit_cast(unsigned, x), b = a;
+    asm volatile("" : "+v"(b));
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
+
 struct AttnKeys {
     const void *K, *V;                       // key head's (and sequence's) first row
     int64_t kst, vst;
@@ -87,6 +97,120 @@ struct AttnKeys {
     bool suffix;
     int b, seen;                             // suffix: its sequence, and suffix_len - Lq + 1: query token i sees seen + i keys
 };
+
+// The whole tiles of a prefix range for 128 rows, 16-bit types: the part where the time goes.  Steps of 32 keys; in step s the
+// VALU turns the scores of s into probabilities while the matrix pipe works out the scores of s + 1, then the products with V run
+// while the maximum of s + 1 is taken; the operands of each product are read from LDS a phase ahead of it.  K is needed a step
+// before V, so the tiles in LDS are K(k + 1) and V(k): each of the two buffers of either is free again a tile before it is needed,
+// and ONE barrier per 64 keys does.  The loads go from global memory to LDS without passing registers (they are issued in the
+// order of the permuted LDS chunks; lanes of columns behind D repeat column 0: their Q is zero and their V is not stored), and have
+// a whole tile's time to arrive.
+template <typename T, int DP>
+__device__ __forceinline__ void attend_whole_tiles(const HpmnPrefixAttn &a, char *lds, const AttnKeys &src, int full,
+                                                   const typename Frag<T>::type (&qf)[DP / 16], float c, float off, float lazy,
+                                                   v16f (&o)[DP / 32], float &m, float &l) {
+    constexpr int KT = 64, CPR = DP / 8, NX = DP / 16, DT = DP / 32, BUF = KT * DP * 2, LD = KT * CPR / 256;
+    typedef typename Frag<T>::type frag;
+    typedef __attribute__((address_space(3))) char lds_char;
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    typedef __attribute__((address_space(3))) frag lds_frag;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, n = lane & 31;
+    lds_char *Kt = (lds_char *)lds, *Vt = Kt + 2 * BUF;
+
+    // global -> LDS: instruction i of wave w fills chunk slots i * 256 + w * 64 + lane
+    const int slot = w * 64 + lane, row = slot / CPR, pos = slot % CPR, col = (chunk_at<CPR>(row, pos) - row * CPR) * 8;
+    const unsigned k_off = (unsigned)(row * src.kst + (col < a.D ? col : 0)) * 2u, v_off = (unsigned)(row * src.vst + (col < a.D ? col : 0)) * 2u;
+    auto dma = [&](lds_char *to, const void *from, int64_t stride, unsigned lane_off, int k0) {
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const T *base = (const T *)from + (k0 + i * (256 / CPR)) * stride;
+            const unsigned at = (unsigned)(uintptr_t)to + i * 4096 + w * 1024;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(lane_off), "s"(base) : "memory", "m0");
+        }
+    };
+    auto load_k = [&](int k) { dma(Kt + (k & 1) * BUF, src.K, src.kst, k_off, src.begin + k * KT); };
+    auto load_v = [&](int k) { dma(Vt + (k & 1) * BUF, src.V, src.vst, v_off, src.begin + k * KT); };
+    auto arrive = [&] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+
+    const int l16 = lane & 15, vrow = 4 * half + (l16 >> 2), vc = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+    frag kf[NX], vf[2][DT];
+    auto read_k = [&](int k, int u) {
+#pragma unroll
+        for (int x = 0; x < NX; ++x) kf[x] = *(const lds_frag *)(Kt + (k & 1) * BUF + 16 * chunk_at<CPR>(32 * u + n, 2 * x + half));
+    };
+    auto read_v = [&](int k, int u) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                union { s16x4 q[2]; frag f; } v;
+                lds_char *at = Vt + (k & 1) * BUF + 8 * (l16 & 1);
+                v.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 16 * chunk_at<CPR>(32 * u + 16 * g + vrow, 4 * t + vc)));
+                v.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 16 * chunk_at<CPR>(32 * u + 16 * g + 8 + vrow, 4 * t + vc)));
+                vf[g][t] = v.f;
+            }
+    };
+    auto raise = [&](const v16f &s, bool real) {
+        float mx = fmaxf(fmaxf(s[0], s[1]), s[2]);
+#pragma unroll
+        for (int i = 3; i < 15; i += 2) mx = fmaxf(fmaxf(mx, s[i]), s[i + 1]);
+        mx = fmaxf(mx, s[15]);
+        mx = fmaxf(mx, other_half(mx)) * c;
+        mx = real ? mx : -FLT_MAX;
+        if (__any(mx > m + lazy)) {
+            const float mn = fmaxf(m, mx), keep = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= keep;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] *= keep;
+        }
+    };
+    // step u of tile k: its scores in `cur`; leaves the scores of the step behind it in `next` and kf for the one behind that
+    auto step = [&](const v16f &cur, v16f &next, int k, int u, bool real) {
+        const float mo = off - m;
+        const v16f zero = {};
+        v8f pf[2];
+        read_v(k, u);
+#pragma unroll
+        for (int x = 0; x < NX; ++x) {
+            next = Frag<T>::mma(kf[x], qf[x], x == 0 ? zero : next);
+#pragma unroll
+            for (int i = x * (16 / NX); i < (x + 1) * (16 / NX); ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(cur[i], c, mo));
+                l += e;
+                pf[i / 8][i % 8] = e;
+            }
+        }
+        read_k(k + 1, u);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const frag pb = __builtin_convertvector(pf[g], frag);
+#pragma unroll
+            for (int t = 0; t < DT; ++t) o[t] = Frag<T>::mma(vf[g][t], pb, o[t]);
+        }
+        raise(next, real);
+    };
+    v16f s0 = {}, s1;
+    attn_barrier();                                          // (the LDS may be in use by the code in front)
+    load_k(0);
+    load_v(0);
+    arrive();
+    if (full > 1) load_k(1);
+    read_k(0, 0);
+#pragma unroll
+    for (int x = 0; x < NX; ++x) s0 = Frag<T>::mma(kf[x], qf[x], s0);
+    read_k(0, 1);
+    raise(s0, true);
+    for (int k = 0; k < full; ++k) {
+        arrive();                                            // K(k + 1) and V(k) are there; K(k) and V(k - 1) have been read by all
+        if (k + 2 < full) load_k(k + 2);
+        if (k + 1 < full) load_v(k + 1);
+        step(s0, s1, k, 0, true);
+        step(s1, s0, k, 1, k + 1 < full);
+    }
+}
 
 template <typename T, int DP, bool VEC, int MW>
 __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &p, char *lds, const AttnKeys &src, int kvh, int row0,
@@ -163,7 +287,7 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
             }
         }
     };
-    auto stage = [&](int k0) {
+    auto stage = [&](int k0, int buf) {
         const bool whole = k0 + KT <= src.end && DP == a.D;
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
@@ -173,8 +297,8 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
                 k = u32x4{0, 0, 0, 0};
                 v = u32x4{0, 0, 0, 0};
             }
-            *(u32x4 *)(Kt + 16 * chunk_at<CPR>(lr, lc)) = k;
-            *(u32x4 *)(Vt + 16 * chunk_at<CPR>(lr, lc)) = v;
+            *(u32x4 *)(Kt + buf + 16 * chunk_at<CPR>(lr, lc)) = k;
+            *(u32x4 *)(Vt + buf + 16 * chunk_at<CPR>(lr, lc)) = v;
         }
     };
 
@@ -185,10 +309,18 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
         for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
     float m = -FLT_MAX, l = 0.f;
 
-    if (src.begin < src.end) fetch(src.begin);
-    for (int k0 = src.begin; k0 < src.end; k0 += KT) {
+    int start = src.begin;
+    if constexpr (!F32 && MW == 4 && VEC) {
+        const int full = (src.end - src.begin) / KT;
+        if (!src.suffix && full > 0 && p.wide) {
+            attend_whole_tiles<T, DP>(a, lds, src, full, qf, c, OFF, LAZY, o, m, l);
+            start = src.begin + full * KT;
+        }
+    }
+    if (start < src.end) fetch(start);
+    for (int k0 = start; k0 < src.end; k0 += KT) {
         attn_barrier();                                  // the last tile has been read
-        stage(k0);
+        stage(k0, 0);
         attn_barrier();
         if (k0 + KT < src.end) fetch(k0 + KT);
         const int kb = kw * 32 * SUB;
@@ -490,15 +622,23 @@ static int attn_rows(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st)
 }
 
 template <typename T>
+static int attn_width(const HpmnPrefixAttn &a, const AttnPlan &p, bool vec, hipStream_t st) {
+    if (a.D <= 32) return vec ? attn_rows<T, 32, true>(a, p, st) : attn_rows<T, 32, false>(a, p, st);
+    if (a.D <= 64) return vec ? attn_rows<T, 64, true>(a, p, st) : attn_rows<T, 64, false>(a, p, st);
+    return vec ? attn_rows<T, 128, true>(a, p, st) : attn_rows<T, 128, false>(a, p, st);
+}
+
+template <typename T>
 int prefix_attn_type(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
     constexpr int E = 16 / sizeof(T);
     bool vec = a.D % E == 0;
     for (const void *q : {a.q, a.k_pre, a.v_pre, a.k_suf, a.v_suf}) vec = vec && is_aligned(q, 16);
     for (int64_t s : {a.q_sb, a.q_sl, a.q_sh, a.kp_st, a.kp_sh, a.vp_st, a.vp_sh, a.ks_sb, a.ks_st, a.ks_sh, a.vs_sb, a.vs_st, a.vs_sh})
         vec = vec && s % E == 0;
-    if (a.D <= 32) return vec ? attn_rows<T, 32, true>(a, p, st) : attn_rows<T, 32, false>(a, p, st);
-    if (a.D <= 64) return vec ? attn_rows<T, 64, true>(a, p, st) : attn_rows<T, 64, false>(a, p, st);
-    return vec ? attn_rows<T, 128, true>(a, p, st) : attn_rows<T, 128, false>(a, p, st);
+    AttnPlan q = p;
+    q.wide = a.kp_st < (1l << 25) && a.vp_st < (1l << 25);   // 64 rows of them in 32 bits of bytes
+    return attn_width<T>(a, q, vec, st);
 }
+
 
 }  // namespace hpmn
