@@ -98,13 +98,16 @@ struct AttnKeys {
     int b, seen;                             // suffix: its sequence, and suffix_len - Lq + 1: query token i sees seen + i keys
 };
 
-// The whole tiles of a prefix range for 128 rows, 16-bit types: the part where the time goes.  Steps of 32 keys; in step s the
-// VALU turns the scores of s into probabilities while the matrix pipe works out the scores of s + 1, then the products with V run
-// while the maximum of s + 1 is taken; the operands of each product are read from LDS a phase ahead of it.  K is needed a step
-// before V, so the tiles in LDS are K(k + 1) and V(k): each of the two buffers of either is free again a tile before it is needed,
-// and ONE barrier per 64 keys does.  The loads go from global memory to LDS without passing registers (they are issued in the
-// order of the permuted LDS chunks; lanes of columns behind D repeat column 0: their Q is zero and their V is not stored), and have
-// a whole tile's time to arrive.
+// The whole tile pairs of a prefix range for 128 rows, 16-bit types: the part where the time goes.  A SIMD overlaps the matrix pipe
+// with the VALU only where ONE wave's instructions alternate (measured: an MFMA with three fma and an exp behind it 36 cycles, alone
+// 32.5; the same work in two waves, each in its own phase: the sum), so every step of 32 keys carries three pipeline stages:
+//   step s:  scores of s + 2 (K Q^T),  products of s (V^T P),  and on the VALU the probabilities of s + 1 and the maximum of s + 2.
+// The maximum raised at the end of step s scales the probabilities from s + 2 on; the output is rescaled a step later, when
+// the products of s + 1 are in it.  Tiles of 64 keys go from global memory to LDS without passing registers (issued in the
+// order of the permuted LDS chunks; lanes of columns behind D repeat column 0: their Q is zero and their V is not stored).  K is
+// needed a tile before V: after the barrier in front of tile k, K(k + 1) and V(k) are there, and the buffers of K(k) and V(k - 1)
+// are free, so two buffers each, one barrier per tile, and a tile's time for the loads.  Tiles go in pairs so that buffers are
+// constants and an LDS address is one of NX + DT registers and an immediate.
 template <typename T, int DP>
 __device__ __forceinline__ void attend_whole_tiles(const HpmnPrefixAttn &a, char *lds, const AttnKeys &src, int full,
                                                    const typename Frag<T>::type (&qf)[DP / 16], float c, float off, float lazy,
@@ -132,83 +135,128 @@ __device__ __forceinline__ void attend_whole_tiles(const HpmnPrefixAttn &a, char
     auto load_v = [&](int k) { dma(Vt + (k & 1) * BUF, src.V, src.vst, v_off, src.begin + k * KT); };
     auto arrive = [&] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
+    // LDS addresses: rows 16 and 32 further and the buffer are immediates (they leave the low four row bits, so the permutation, alone)
     const int l16 = lane & 15, vrow = 4 * half + (l16 >> 2), vc = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
-    frag kf[NX], vf[2][DT];
-    auto read_k = [&](int k, int u) {
+    lds_char *ka[NX], *va[DT][2];
 #pragma unroll
-        for (int x = 0; x < NX; ++x) kf[x] = *(const lds_frag *)(Kt + (k & 1) * BUF + 16 * chunk_at<CPR>(32 * u + n, 2 * x + half));
+    for (int x = 0; x < NX; ++x) ka[x] = Kt + 16 * chunk_at<CPR>(n, 2 * x + half);
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) va[t][j] = Vt + 16 * chunk_at<CPR>(vrow + 8 * j, 4 * t + vc) + 8 * (l16 & 1);
+    auto scores = [&](int buf, int u) {
+        v16f s = {};
+#pragma unroll
+        for (int x = 0; x < NX; ++x) s = Frag<T>::mma(*(const lds_frag *)(ka[x] + buf * BUF + 32 * u * CPR * 16), qf[x], s);
+        return s;
     };
-    auto read_v = [&](int k, int u) {
+    auto top = [&](const v16f &s) {
+        float mx = fmaxf(fmaxf(s[0], s[1]), s[2]);
+#pragma unroll
+        for (int i = 3; i < 15; i += 2) mx = fmaxf(fmaxf(mx, s[i]), s[i + 1]);
+        mx = fmaxf(mx, s[15]);
+        return fmaxf(mx, other_half(mx)) * c;
+    };
+    float pending = 1.f;                     // what the output still has to be multiplied with
+    auto settle_output = [&](float pending) {
+        if (__any(pending != 1.f)) {
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] *= pending;
+        }
+    };
+    auto raise = [&](float mx) {             // (no branch: it is on the way of the interleaved instructions)
+        const float mn = mx > m + lazy ? mx : m;
+        pending = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= pending;
+    };
+    auto probabilities = [&](const v16f &s, frag (&p)[2]) {
+        const float mo = off - m;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            v8f e;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                e[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * g + i], c, mo));
+                l += e[i];
+            }
+            p[g] = __builtin_convertvector(e, frag);
+        }
+    };
+    // step (buffer vb, u): s1: scores of the next step, turned into p1; p0: this step's probabilities; leaves the scores of the step
+    // after next in s2
+    auto step = [&](int vb, int kb, int u, const frag (&p0)[2], const v16f &s1, frag (&p1)[2], v16f &s2, float cap) {
+        frag kf[NX], vf[2][DT];
+        v16f cur = s1;
+        asm volatile("" : "+v"(cur));        // (nothing of this step moves in front of it)
+#pragma unroll
+        for (int x = 0; x < NX; ++x) kf[x] = *(const lds_frag *)(ka[x] + kb * BUF + 32 * u * CPR * 16);
 #pragma unroll
         for (int g = 0; g < 2; ++g)
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
                 union { s16x4 q[2]; frag f; } v;
-                lds_char *at = Vt + (k & 1) * BUF + 8 * (l16 & 1);
-                v.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 16 * chunk_at<CPR>(32 * u + 16 * g + vrow, 4 * t + vc)));
-                v.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 16 * chunk_at<CPR>(32 * u + 16 * g + 8 + vrow, 4 * t + vc)));
+                const int at = vb * BUF + (32 * u + 16 * g) * CPR * 16;
+                v.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(va[t][0] + at));
+                v.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(va[t][1] + at));
                 vf[g][t] = v.f;
             }
-    };
-    auto raise = [&](const v16f &s, bool real) {
-        float mx = fmaxf(fmaxf(s[0], s[1]), s[2]);
+        probabilities(cur, p1);
+        v16f s = {};
 #pragma unroll
-        for (int i = 3; i < 15; i += 2) mx = fmaxf(fmaxf(mx, s[i]), s[i + 1]);
-        mx = fmaxf(mx, s[15]);
-        mx = fmaxf(mx, other_half(mx)) * c;
-        mx = real ? mx : -FLT_MAX;
-        if (__any(mx > m + lazy)) {
-            const float mn = fmaxf(m, mx), keep = __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= keep;
+        for (int x = 0; x < NX; ++x) s = Frag<T>::mma(kf[x], qf[x], s);
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
+        for (int g = 0; g < 2; ++g)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[t][i] *= keep;
-        }
-    };
-    // step u of tile k: its scores in `cur`; leaves the scores of the step behind it in `next` and kf for the one behind that
-    auto step = [&](const v16f &cur, v16f &next, int k, int u, bool real) {
-        const float mo = off - m;
-        const v16f zero = {};
-        v8f pf[2];
-        read_v(k, u);
+            for (int t = 0; t < DT; ++t) o[t] = Frag<T>::mma(vf[g][t], p0[g], o[t]);
+        s2 = s;
+        const float mx = fminf(top(s), cap);     // (cap: whether the step after next exists; no branch)
+        const float scale_out = pending;
+        raise(mx);
+        asm volatile("" : "+v"(p1[0]), "+v"(p1[1]), "+v"(m), "+v"(l));              // (and nothing is left for later)
+        // the order: both operand sets from LDS, then an MFMA and a share of the VALU work in turn
+        __builtin_amdgcn_sched_group_barrier(0x100, NX, 0);
 #pragma unroll
         for (int x = 0; x < NX; ++x) {
-            next = Frag<T>::mma(kf[x], qf[x], x == 0 ? zero : next);
-#pragma unroll
-            for (int i = x * (16 / NX); i < (x + 1) * (16 / NX); ++i) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(cur[i], c, mo));
-                l += e;
-                pf[i / 8][i % 8] = e;
-            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 4 * DT / NX, 0);
+            __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
         }
-        read_k(k + 1, u);
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            const frag pb = __builtin_convertvector(pf[g], frag);
-#pragma unroll
-            for (int t = 0; t < DT; ++t) o[t] = Frag<T>::mma(vf[g][t], pb, o[t]);
+        for (int x = 0; x < 2 * DT; ++x) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
         }
-        raise(next, real);
+        settle_output(scale_out);
     };
-    v16f s0 = {}, s1;
     attn_barrier();                                          // (the LDS may be in use by the code in front)
     load_k(0);
     load_v(0);
+    load_k(1);
     arrive();
-    if (full > 1) load_k(1);
-    read_k(0, 0);
-#pragma unroll
-    for (int x = 0; x < NX; ++x) s0 = Frag<T>::mma(kf[x], qf[x], s0);
-    read_k(0, 1);
-    raise(s0, true);
-    for (int k = 0; k < full; ++k) {
+    v16f sa = scores(0, 0), sb = scores(0, 1);
+    frag pa[2], pb[2];
+    raise(top(sa));                                          // (the output is still zero)
+    probabilities(sa, pa);
+    raise(top(sb));
+    for (int k = 0; k < full; k += 2) {
         arrive();                                            // K(k + 1) and V(k) are there; K(k) and V(k - 1) have been read by all
         if (k + 2 < full) load_k(k + 2);
-        if (k + 1 < full) load_v(k + 1);
-        step(s0, s1, k, 0, true);
-        step(s1, s0, k, 1, k + 1 < full);
+        load_v(k + 1);
+        step(0, 1, 0, pa, sb, pb, sa, FLT_MAX);
+        step(0, 1, 1, pb, sa, pa, sb, FLT_MAX);
+        arrive();
+        if (k + 3 < full) load_k(k + 3);
+        if (k + 2 < full) load_v(k + 2);
+        const float cap = k + 2 < full ? FLT_MAX : -FLT_MAX;
+        step(1, 0, 0, pa, sb, pb, sa, cap);
+        const float before = l;
+        step(1, 0, 1, pb, sa, pa, sb, cap);
+        if (k + 2 >= full) l = before;       // (there was no next step whose probabilities could count)
     }
 }
 
@@ -311,7 +359,7 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
 
     int start = src.begin;
     if constexpr (!F32 && MW == 4 && VEC) {
-        const int full = (src.end - src.begin) / KT;
+        const int full = (src.end - src.begin) / (2 * KT) * 2;
         if (!src.suffix && full > 0 && p.wide) {
             attend_whole_tiles<T, DP>(a, lds, src, full, qf, c, OFF, LAZY, o, m, l);
             start = src.begin + full * KT;

@@ -19,16 +19,17 @@ AttnPlan attn_plan(const HpmnPrefixAttn &a) {
     p.mw_suf = per_seq > 64 ? 4 : few;
     auto split = [&](long base, int keys, int tile, int &splits, int &per) {
         const int tiles = std::max(1, (keys + tile - 1) / tile);
-        // one workgroup per CU, two when each still has 20 tiles to work through (a tile's loads hide behind the other's products;
+        // one workgroup per CU, two when each still has 1280 keys to work through (a tile's loads hide behind the other's products;
         // shorter ranges pay more for their start and for the join): 300 x 8 heads of 128, 16384 keys 54 -> 50 us with two,
         // 200 x 8 heads over 2 of 64, 4096 keys 17.5 -> 21 us
         splits = (int)std::max<long>(1, std::min<long>(tiles, 256 / base));
-        if (tiles / splits >= 20) splits = (int)std::max<long>(1, std::min<long>(tiles, 512 / base));
+        if ((long)tiles * tile / splits >= 1280) splits = (int)std::max<long>(1, std::min<long>(tiles, 512 / base));
         per = (tiles + splits - 1) / splits * tile;
         splits = std::max(1, (keys + per - 1) / per);
     };
     p.rt_pre = (int)((M + 32 * p.mw_pre - 1) / (32 * p.mw_pre));
-    split((long)p.rt_pre * a.Hkv, a.P, attn_tile(esize, p.mw_pre), p.splits_pre, p.per_pre);
+    // (16-bit, many rows: pairs of tiles)
+    split((long)p.rt_pre * a.Hkv, a.P, attn_tile(esize, p.mw_pre) * (esize == 2 && p.mw_pre == 4 ? 2 : 1), p.splits_pre, p.per_pre);
     p.blocks_pre = (unsigned)(((long)a.Hkv * p.splits_pre + 7) / 8 * 8 * p.rt_pre);
     if (a.S > 0) {
         p.rt_suf = (int)((per_seq + 32 * p.mw_suf - 1) / (32 * p.mw_suf));
