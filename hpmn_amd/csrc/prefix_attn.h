@@ -2,15 +2,15 @@
 // instantiates it: prefix_attn.hip, prefix_attn_bf16.hip, prefix_attn_f16.hip).
 //
 // The query rows of one key head -- every (sequence, query token, grouped head) -- are a matrix of M = B Lq Hq / Hkv rows against the
-// SAME prefix, so the prefix is a matrix product's operand: a workgroup takes 128 rows (or 32, when there are few) and a range of
+// SAME prefix, so the prefix is a matrix product's operand: a workgroup takes 128 rows (or 64 or 32, when there are few) and a range of
 // keys, and K and V are read once per 128 rows instead of once per row.  One pass with the running maximum and sum:
 //   S^T = K Q^T   a wave: 32 query rows (columns of S^T: one row per lane pair, so maximum and sum are a register reduction and ONE
 //                 exchange between the wave's halves), 32 keys at a time on the matrix pipe, Q in registers throughout;
 //   O^T += V^T P  P is used where it lies: S^T's accumulator layout is the operand layout of the second product up to an order of
 //                 the keys, and V is read in that order (16-bit: transposing LDS reads, four keys x 16 columns per 16 lanes).
-// K and V tiles go global -> registers -> LDS, the next tile in flight while this one is used; LDS chunks of 16 bytes are permuted
-// by the row number so that neither the reads along a row nor those across eight rows meet in a bank.
-// Few rows: the four waves of a workgroup share out the keys of a tile instead of the rows and join their results in LDS.  The key
+// K and V tiles go from global memory to LDS directly, the next tile in flight while this one is used; LDS chunks of 16 bytes are
+// permuted by the row number so that neither the reads along a row nor those across sixteen rows meet in a bank.
+// Few rows: two or all four waves of a workgroup share out the keys of a tile and join their results in LDS.  The key
 // axis is split over workgroups until the chip is full; a second kernel joins the parts (maximum, sum, unnormalised output in fp32).
 // A row's own suffix is the same thing with M = Lq Hq / Hkv rows and a key limit per row, in the same launch.
 //
@@ -33,7 +33,6 @@ struct AttnPlan {
     int parts;                               // splits_pre + splits_suf; 1: no second kernel, results go straight out
     int d4;                                  // D rounded up to 4: a row of a part
     long rows;                               // Hkv * M
-    int wide;                                // the prefix's row strides fit attend_whole_tiles (32-bit lane offsets)
     long o_at;                               // where the parts' outputs start in the workspace, in floats (behind their m and l)
     unsigned blocks_pre, blocks_suf;
 };
@@ -46,7 +45,7 @@ constexpr int attn_sub(int esize, int mw) { return esize == 2 && mw == 4 ? 2 : 1
 constexpr int attn_tile(int esize, int mw) { return 4 / mw * 32 * attn_sub(esize, mw); }
 constexpr size_t attn_lds(int esize, int dp, int mw) {
     const size_t tiles = (size_t)2 * attn_tile(esize, mw) * dp * esize, join = (size_t)4 * 32 * (dp + 4) * 4 + 4 * 32 * 8;
-    return mw == 4 ? (esize == 2 ? 2 * tiles : tiles) : std::max(tiles, join);
+    return mw == 4 ? 2 * tiles : std::max(2 * tiles, join);
 }
 
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -98,13 +97,59 @@ struct AttnKeys {
     int b, seen;                             // suffix: its sequence, and suffix_len - Lq + 1: query token i sees seen + i keys
 };
 
+// Tiles from global memory to LDS without passing registers: instruction i of wave w fills the 64 chunk slots from i * 256 + w * 64 on,
+// slot by slot, so a lane picks the chunk that belongs into its slot.  Columns behind D repeat column 0 (their Q is zero, their V is
+// not stored).  Row strides below 2^24 elements: a tile's lane offsets fit 32 bits.
+template <typename T, int DP, int KT>
+struct TileLoader {
+    static constexpr int EPC = 16 / sizeof(T), CPR = DP / EPC, LD = KT * CPR / 256, ROWS = 256 / CPR;
+    static constexpr int ALT = ROWS < 16 ? 2 : 1;            // the permutation goes by the low four row bits: every other instruction's
+    int row, col[ALT], w;
+    unsigned k_off[ALT], v_off[ALT];
+    __device__ __forceinline__ TileLoader(const HpmnPrefixAttn &a, const AttnKeys &src) {
+        w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int slot = threadIdx.x;
+        row = slot / CPR;
+#pragma unroll
+        for (int j = 0; j < ALT; ++j) {
+            col[j] = (chunk_at<CPR>(row + j * ROWS, slot % CPR) - (row + j * ROWS) * CPR) * EPC;
+            if (col[j] >= a.D) col[j] = 0;
+            k_off[j] = (unsigned)(row * src.kst + col[j]) * (unsigned)sizeof(T);
+            v_off[j] = (unsigned)(row * src.vst + col[j]) * (unsigned)sizeof(T);
+        }
+    }
+    // rows k0 .. k0 + KT of `from` (all of them there)
+    __device__ __forceinline__ void whole(unsigned lds, const void *from, int64_t stride, const unsigned (&lane_off)[ALT], int k0) const {
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const T *base = (const T *)from + (k0 + i * ROWS) * stride;
+            const unsigned at = lds + i * 4096 + w * 1024;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(lane_off[i % ALT]), "s"(base) : "memory", "m0");
+        }
+    }
+    // rows behind `end` repeat the last one
+    __device__ __forceinline__ void partial(unsigned lds, const void *from, int64_t stride, int k0, int end) const {
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const T *at_row = (const T *)from + min(k0 + row + i * ROWS, end - 1) * stride + col[i % ALT];
+            const unsigned at = lds + i * 4096 + w * 1024;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(at_row) : "memory", "m0");
+        }
+    }
+    __device__ __forceinline__ void load(unsigned lds, const void *from, int64_t stride, const unsigned (&lane_off)[ALT], int k0, int end) const {
+        if (k0 + KT <= end) whole(lds, from, stride, lane_off, k0);
+        else partial(lds, from, stride, k0, end);
+    }
+};
+// The loads of this wave have arrived, and then those of all.
+__device__ __forceinline__ void attn_arrive() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // The whole tile pairs of a prefix range for 128 rows, 16-bit types: the part where the time goes.  A SIMD overlaps the matrix pipe
 // with the VALU only where ONE wave's instructions alternate (measured: an MFMA with three fma and an exp behind it 36 cycles, alone
 // 32.5; the same work in two waves, each in its own phase: the sum), so every step of 32 keys carries three pipeline stages:
 //   step s:  scores of s + 2 (K Q^T),  products of s (V^T P),  and on the VALU the probabilities of s + 1 and the maximum of s + 2.
 // The maximum raised at the end of step s scales the probabilities from s + 2 on; the output is rescaled a step later, when
-// the products of s + 1 are in it.  Tiles of 64 keys go from global memory to LDS without passing registers (issued in the
-// order of the permuted LDS chunks; lanes of columns behind D repeat column 0: their Q is zero and their V is not stored).  K is
+// the products of s + 1 are in it.  Tiles of 64 keys.  K is
 // needed a tile before V: after the barrier in front of tile k, K(k + 1) and V(k) are there, and the buffers of K(k) and V(k - 1)
 // are free, so two buffers each, one barrier per tile, and a tile's time for the loads.  Tiles go in pairs so that buffers are
 // constants and an LDS address is one of NX + DT registers and an immediate.
@@ -112,28 +157,18 @@ template <typename T, int DP>
 __device__ __forceinline__ void attend_whole_tiles(const HpmnPrefixAttn &a, char *lds, const AttnKeys &src, int full,
                                                    const typename Frag<T>::type (&qf)[DP / 16], float c, float off, float lazy,
                                                    v16f (&o)[DP / 32], float &m, float &l) {
-    constexpr int KT = 64, CPR = DP / 8, NX = DP / 16, DT = DP / 32, BUF = KT * DP * 2, LD = KT * CPR / 256;
+    constexpr int KT = 64, CPR = DP / 8, NX = DP / 16, DT = DP / 32, BUF = KT * DP * 2;
     typedef typename Frag<T>::type frag;
     typedef __attribute__((address_space(3))) char lds_char;
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     typedef __attribute__((address_space(3))) frag lds_frag;
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, n = lane & 31;
+    const int lane = threadIdx.x & 63, half = lane >> 5, n = lane & 31;
     lds_char *Kt = (lds_char *)lds, *Vt = Kt + 2 * BUF;
 
-    // global -> LDS: instruction i of wave w fills chunk slots i * 256 + w * 64 + lane
-    const int slot = w * 64 + lane, row = slot / CPR, pos = slot % CPR, col = (chunk_at<CPR>(row, pos) - row * CPR) * 8;
-    const unsigned k_off = (unsigned)(row * src.kst + (col < a.D ? col : 0)) * 2u, v_off = (unsigned)(row * src.vst + (col < a.D ? col : 0)) * 2u;
-    auto dma = [&](lds_char *to, const void *from, int64_t stride, unsigned lane_off, int k0) {
-#pragma unroll
-        for (int i = 0; i < LD; ++i) {
-            const T *base = (const T *)from + (k0 + i * (256 / CPR)) * stride;
-            const unsigned at = (unsigned)(uintptr_t)to + i * 4096 + w * 1024;
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(lane_off), "s"(base) : "memory", "m0");
-        }
-    };
-    auto load_k = [&](int k) { dma(Kt + (k & 1) * BUF, src.K, src.kst, k_off, src.begin + k * KT); };
-    auto load_v = [&](int k) { dma(Vt + (k & 1) * BUF, src.V, src.vst, v_off, src.begin + k * KT); };
-    auto arrive = [&] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    const TileLoader<T, DP, KT> loader(a, src);
+    const unsigned lds0 = (unsigned)(uintptr_t)Kt;
+    auto load_k = [&](int k) { loader.whole(lds0 + (k & 1) * BUF, src.K, src.kst, loader.k_off, src.begin + k * KT); };
+    auto load_v = [&](int k) { loader.whole(lds0 + (2 + (k & 1)) * BUF, src.V, src.vst, loader.v_off, src.begin + k * KT); };
 
     // LDS addresses: rows 16 and 32 further and the buffer are immediates (they leave the low four row bits, so the permutation, alone)
     const int l16 = lane & 15, vrow = 4 * half + (l16 >> 2), vc = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
@@ -237,19 +272,19 @@ __device__ __forceinline__ void attend_whole_tiles(const HpmnPrefixAttn &a, char
     load_k(0);
     load_v(0);
     load_k(1);
-    arrive();
+    attn_arrive();
     v16f sa = scores(0, 0), sb = scores(0, 1);
     frag pa[2], pb[2];
     raise(top(sa));                                          // (the output is still zero)
     probabilities(sa, pa);
     raise(top(sb));
     for (int k = 0; k < full; k += 2) {
-        arrive();                                            // K(k + 1) and V(k) are there; K(k) and V(k - 1) have been read by all
+        attn_arrive();                                       // K(k + 1) and V(k) are there; K(k) and V(k - 1) have been read by all
         if (k + 2 < full) load_k(k + 2);
         load_v(k + 1);
         step(0, 1, 0, pa, sb, pb, sa, FLT_MAX);
         step(0, 1, 1, pb, sa, pa, sb, FLT_MAX);
-        arrive();
+        attn_arrive();
         if (k + 3 < full) load_k(k + 3);
         if (k + 2 < full) load_v(k + 2);
         const float cap = k + 2 < full ? FLT_MAX : -FLT_MAX;
@@ -269,7 +304,8 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
     constexpr float OFF = std::is_same<T, f16_t>::value ? 15.f : 0.f;
     constexpr float LAZY = OFF > 0.f ? 0.f : 8.f;       // the maximum may lag by 2^LAZY before O is rescaled
     typedef typename Frag<T>::type frag;
-    char *Kt = lds, *Vt = lds + KT * DP * (int)sizeof(T);
+    constexpr int BUF = 2 * KT * DP * (int)sizeof(T);    // K and V of a tile; two of them
+    char *Kt = lds, *Vt = lds + BUF / 2;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, n = lane & 31;
     const int mw = w % MW, kw = w / MW;
     const int group = a.Hq / a.Hkv, per_seq = a.Lq * group;
@@ -309,44 +345,34 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
     }
     const float c = a.scale == 0.f ? 1.f : -NEG_LOG2E * fabsf(a.scale);
 
-    // this thread's chunks of a tile: one column of chunks, rows 256 / CPR apart
+    // What no 16-byte access can take (VEC false): element by element through registers, the next tile in flight.  This thread's
+    // chunks: one column of chunks, rows 256 / CPR apart.
     const int lc = tid % CPR, lrow = tid / CPR;
-    u32x4 kr[LD], vr[LD];
+    u32x4 kr[VEC ? 1 : LD], vr[VEC ? 1 : LD];
     auto fetch = [&](int k0) {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             const int key = min(k0 + lrow + i * (256 / CPR), src.end - 1);
             const T *k = (const T *)src.K + key * src.kst, *v = (const T *)src.V + key * src.vst;
-            if constexpr (VEC) {
-                const int d = lc * EPC < a.D ? lc * EPC : 0;
-                kr[i] = *(const u32x4 *)(k + d);
-                vr[i] = *(const u32x4 *)(v + d);
-            } else {
-                union { T e[EPC]; u32x4 u; } x, y;
+            union { T e[EPC]; u32x4 u; } x, y;
 #pragma unroll
-                for (int e = 0; e < EPC; ++e) {
-                    const int d = lc * EPC + e;
-                    const T ke = k[min(d, a.D - 1)], ve = v[min(d, a.D - 1)];
-                    x.e[e] = d < a.D ? ke : (T)0.f;
-                    y.e[e] = d < a.D ? ve : (T)0.f;
-                }
-                kr[i] = x.u;
-                vr[i] = y.u;
+            for (int e = 0; e < EPC; ++e) {
+                const int d = lc * EPC + e;
+                const T ke = k[min(d, a.D - 1)], ve = v[min(d, a.D - 1)];
+                x.e[e] = d < a.D ? ke : (T)0.f;
+                y.e[e] = d < a.D ? ve : (T)0.f;
             }
+            kr[i] = x.u;
+            vr[i] = y.u;
         }
     };
     auto stage = [&](int k0, int buf) {
-        const bool whole = k0 + KT <= src.end && DP == a.D;
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             const int lr = lrow + i * (256 / CPR);
-            u32x4 k = kr[i], v = vr[i];
-            if (!whole && (k0 + lr >= src.end || (VEC && lc * EPC >= a.D))) {   // (zeros, not what lies there: 0 * NaN)
-                k = u32x4{0, 0, 0, 0};
-                v = u32x4{0, 0, 0, 0};
-            }
-            *(u32x4 *)(Kt + buf + 16 * chunk_at<CPR>(lr, lc)) = k;
-            *(u32x4 *)(Vt + buf + 16 * chunk_at<CPR>(lr, lc)) = v;
+            const bool there = k0 + lr < src.end;            // (zeros, not what lies there: 0 * NaN)
+            *(u32x4 *)(Kt + buf + 16 * chunk_at<CPR>(lr, lc)) = there ? kr[i] : u32x4{0, 0, 0, 0};
+            *(u32x4 *)(Vt + buf + 16 * chunk_at<CPR>(lr, lc)) = there ? vr[i] : u32x4{0, 0, 0, 0};
         }
     };
 
@@ -360,19 +386,50 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
     int start = src.begin;
     if constexpr (!F32 && MW == 4 && VEC) {
         const int full = (src.end - src.begin) / (2 * KT) * 2;
-        if (!src.suffix && full > 0 && p.wide) {
+        if (!src.suffix && full > 0) {
             attend_whole_tiles<T, DP>(a, lds, src, full, qf, c, OFF, LAZY, o, m, l);
             start = src.begin + full * KT;
         }
     }
-    if (start < src.end) fetch(start);
-    for (int k0 = start; k0 < src.end; k0 += KT) {
-        attn_barrier();                                  // the last tile has been read
-        stage(k0, 0);
-        attn_barrier();
-        if (k0 + KT < src.end) fetch(k0 + KT);
+    const TileLoader<T, DP, KT> loader(a, src);
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    auto load = [&](int k0, int buf) {
+        loader.load(lds0 + buf, src.K, src.kst, loader.k_off, k0, src.end);
+        loader.load(lds0 + buf + BUF / 2, src.V, src.vst, loader.v_off, k0, src.end);
+    };
+    int buf = 0;
+    if (start < src.end) {
+        attn_barrier();                                      // (the LDS may be in use by the code in front)
+        if constexpr (VEC) {
+            load(start, 0);
+        } else {
+            fetch(start);
+            stage(start, 0);
+        }
+    }
+    for (int k0 = start; k0 < src.end; k0 += KT, buf ^= BUF) {
+        // this tile is there, and the last one, whose buffer the next one takes, has been read by all
+        if constexpr (VEC) {
+            attn_arrive();
+            if (k0 + KT < src.end) load(k0 + KT, buf ^ BUF);
+            else if (k0 + KT > src.end) {                    // V behind the end: zeros, not repeated rows (0 * inf)
+                for (int i = tid; i < (k0 + KT - src.end) * CPR; i += 256)
+                    *(u32x4 *)(Vt + buf + 16 * (src.end - k0) * CPR + 16 * i) = u32x4{0, 0, 0, 0};
+                attn_barrier();
+            }
+        } else {
+            attn_barrier();
+            if (k0 + KT < src.end) fetch(k0 + KT);
+        }
+        const auto last = [&] {                              // (registers to LDS once this tile has been used)
+            if constexpr (!VEC)
+                if (k0 + KT < src.end) stage(k0 + KT, buf ^ BUF);
+        };
         const int kb = kw * 32 * SUB;
-        if (!active || k0 + kb >= src.end) continue;
+        if (!active || k0 + kb >= src.end) {
+            last();
+            continue;
+        }
         v16f s[SUB];
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
@@ -380,7 +437,7 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
             for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
 #pragma unroll
             for (int x = 0; x < DP / (2 * EPC); ++x) {
-                const frag kf = *(const frag *)(Kt + 16 * chunk_at<CPR>(kb + 32 * u + n, 2 * x + half));
+                const frag kf = *(const frag *)(Kt + buf + 16 * chunk_at<CPR>(kb + 32 * u + n, 2 * x + half));
                 if constexpr (F32) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], qf[x][e], s[u], 0, 0, 0);
@@ -401,7 +458,7 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32)) * c;
+        mx = fmaxf(mx, other_half(mx)) * c;
         if (__any(mx > m + LAZY)) {
             const float mn = fmaxf(m, mx), keep = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
@@ -426,7 +483,7 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
 #pragma unroll
                     for (int t = 0; t < DT; ++t) {
                         const int d = 32 * t + n;
-                        const float v = *(const float *)(Vt + 16 * chunk_at<CPR>(vrow, d / 4) + 4 * (d % 4));
+                        const float v = *(const float *)(Vt + buf + 16 * chunk_at<CPR>(vrow, d / 4) + 4 * (d % 4));
                         o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[u][i], o[t], 0, 0, 0);
                     }
                 }
@@ -442,13 +499,14 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
 #pragma unroll
                     for (int t = 0; t < DT; ++t) {
                         union { s16x4 q[2]; frag f; } x;
-                        x.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(Vt + 16 * chunk_at<CPR>(vr0 + 16 * g, 4 * t + vc) + 8 * (l16 & 1)));
-                        x.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(Vt + 16 * chunk_at<CPR>(vr0 + 16 * g + 8, 4 * t + vc) + 8 * (l16 & 1)));
+                        x.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(Vt + buf + 16 * chunk_at<CPR>(vr0 + 16 * g, 4 * t + vc) + 8 * (l16 & 1)));
+                        x.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(Vt + buf + 16 * chunk_at<CPR>(vr0 + 16 * g + 8, 4 * t + vc) + 8 * (l16 & 1)));
                         o[t] = Frag<T>::mma(x.f, pb, o[t]);
                     }
                 }
             }
         }
+        last();
     }
     l += __shfl_xor(l, 32);
     m -= OFF;
@@ -524,7 +582,7 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
 }
 
 template <typename T, int DP, bool VEC, int MWP, int MWS>
-__global__ __launch_bounds__(256, 2) void prefix_attn_kernel(const HpmnPrefixAttn a, const AttnPlan p) {
+__global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128) ? 1 : 2) void prefix_attn_kernel(const HpmnPrefixAttn a, const AttnPlan p) {
     extern __shared__ char attn_smem[];
     const int group = a.Hq / a.Hkv;
     AttnKeys k;
@@ -664,9 +722,10 @@ static int attn_go(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
 
 template <typename T, int DP, bool VEC>
 static int attn_rows(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
-    constexpr int FEW = sizeof(T) == 4 ? 2 : 1;
-    if (p.mw_pre != 4) return attn_go<T, DP, VEC, FEW, FEW>(a, p, st);
-    return p.mw_suf == 4 ? attn_go<T, DP, VEC, 4, 4>(a, p, st) : attn_go<T, DP, VEC, 4, FEW>(a, p, st);
+    if (p.mw_pre == 4) return p.mw_suf == 4 ? attn_go<T, DP, VEC, 4, 4>(a, p, st) : attn_go<T, DP, VEC, 4, 2>(a, p, st);
+    if constexpr (sizeof(T) == 2)
+        if (p.mw_pre == 1) return attn_go<T, DP, VEC, 1, 2>(a, p, st);
+    return attn_go<T, DP, VEC, 2, 2>(a, p, st);
 }
 
 template <typename T>
@@ -683,9 +742,8 @@ int prefix_attn_type(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st)
     for (const void *q : {a.q, a.k_pre, a.v_pre, a.k_suf, a.v_suf}) vec = vec && is_aligned(q, 16);
     for (int64_t s : {a.q_sb, a.q_sl, a.q_sh, a.kp_st, a.kp_sh, a.vp_st, a.vp_sh, a.ks_sb, a.ks_st, a.ks_sh, a.vs_sb, a.vs_st, a.vs_sh})
         vec = vec && s % E == 0;
-    AttnPlan q = p;
-    q.wide = a.kp_st < (1l << 25) && a.vp_st < (1l << 25);   // 64 rows of them in 32 bits of bytes
-    return attn_width<T>(a, q, vec, st);
+    for (int64_t s : {a.kp_st, a.vp_st, a.ks_st, a.vs_st}) vec = vec && s < (1l << 24);      // TileLoader: 128 rows in 32 bits of bytes
+    return attn_width<T>(a, p, vec, st);
 }
 
 

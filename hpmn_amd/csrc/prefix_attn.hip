@@ -7,23 +7,24 @@ namespace hpmn {
 extern template int prefix_attn_type<bf16_t>(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st);
 extern template int prefix_attn_type<f16_t>(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st);
 
-// By sizes and type alone.  Rows: 128 per workgroup from 65 on (below, the waves share out keys).  Keys: split until about two
+// By sizes and type alone.  Rows: 128 per workgroup from 65 on (below, the waves share out keys; four ways only for 16-bit types,
+// whose tiles leave room for it: 8 x 8 heads over 1 of 64, 32768 keys 16.3 us against 21.3 two ways).  Keys: split until about two
 // workgroups per CU exist.
 AttnPlan attn_plan(const HpmnPrefixAttn &a) {
     AttnPlan p = {};
-    const int esize = (int)elem_size(a.dtype), few = esize == 4 ? 2 : 1, group = a.Hq / a.Hkv;
+    const int esize = (int)elem_size(a.dtype), group = a.Hq / a.Hkv;
     const long M = (long)a.B * a.Lq * group, per_seq = (long)a.Lq * group;
     p.rows = M * a.Hkv;
     p.d4 = (a.D + 3) / 4 * 4;
-    p.mw_pre = M > 64 ? 4 : few;
-    p.mw_suf = per_seq > 64 ? 4 : few;
+    p.mw_pre = M > 64 ? 4 : M > 32 || esize == 4 ? 2 : 1;
+    p.mw_suf = per_seq > 64 ? 4 : 2;
     auto split = [&](long base, int keys, int tile, int &splits, int &per) {
         const int tiles = std::max(1, (keys + tile - 1) / tile);
-        // one workgroup per CU, two when each still has 1280 keys to work through (a tile's loads hide behind the other's products;
+        // one workgroup per CU, two when each still has 1280 keys (fp32: 320) to work through (a tile's loads hide behind the other's products;
         // shorter ranges pay more for their start and for the join): 300 x 8 heads of 128, 16384 keys 54 -> 50 us with two,
         // 200 x 8 heads over 2 of 64, 4096 keys 17.5 -> 21 us
         splits = (int)std::max<long>(1, std::min<long>(tiles, 256 / base));
-        if ((long)tiles * tile / splits >= 1280) splits = (int)std::max<long>(1, std::min<long>(tiles, 512 / base));
+        if ((long)tiles * tile / splits >= (esize == 4 ? 320 : 1280)) splits = (int)std::max<long>(1, std::min<long>(tiles, 512 / base));
         per = (tiles + splits - 1) / splits * tile;
         splits = std::max(1, (keys + per - 1) / per);
     };
