@@ -625,66 +625,74 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128) ? 1 : 2) void pr
     }
 }
 
-// Second kernel: joins a row's parts.  Groups of 32 lanes (a quad of the row each, D <= 128) take the parts in turn; BLOCK: a
-// workgroup of eight groups per row, else a wave of two.  The weights of the first 64 parts of a group's turn are worked out side
-// by side in the lanes first, so that the loop over the parts is loads that depend on nothing.
-template <typename T, bool BLOCK>
+// Second kernel: joins a row's parts.  Groups of 32 lanes (a quad of the row each, D <= 128) take the parts in turn, BATCH at a
+// time; BLOCK: a workgroup of eight groups per row, else a wave of two.  What the parts hold was written by other XCDs, a round trip to
+// memory is most of this kernel: a batch's outputs are asked for before its weights are known, and both in one go.
+template <typename T, bool BLOCK, int BATCH>
 __global__ __launch_bounds__(256) void prefix_attn_join_kernel(const HpmnPrefixAttn a, const AttnPlan p) {
     constexpr int GROUPS = BLOCK ? 8 : 2;
-    __shared__ float top[4];
-    __shared__ v4f sums[BLOCK ? 8 : 1][32];
-    __shared__ float ls[8];
+    __shared__ v4f sums[8][32];
+    __shared__ float ls[8], ms[8];
     const long R = BLOCK ? (long)blockIdx.x : (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (R >= p.rows) return;                             // (whole waves; BLOCK: never)
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane & 31, grp = BLOCK ? (int)threadIdx.x >> 5 : lane >> 5;
+    const int lane = threadIdx.x & 63, q = lane & 31, grp = BLOCK ? (int)threadIdx.x >> 5 : lane >> 5;
     const float *ml = (const float *)a.workspace, *parts = ml + p.o_at;
-    float m = -FLT_MAX;
-    for (int k = BLOCK ? (int)threadIdx.x : lane; k < p.parts; k += BLOCK ? 256 : 64) {
-        const float mk = ml[(k * p.rows + R) * 2], lk = ml[(k * p.rows + R) * 2 + 1];
-        m = fmaxf(m, lk != 0.f ? mk : -FLT_MAX);
-    }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    if (BLOCK) {
-        if (lane == 0) top[w] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-    }
-    float l = 0.f;
-    v4f x = {0.f, 0.f, 0.f, 0.f};
     const int d0 = min(4 * q, p.d4 - 4);
-    for (int k0 = grp; k0 < p.parts; k0 += 32 * GROUPS) {
-        const int mine = k0 + q * GROUPS;                // lane q of the group: the weight of the turn's q-th part
-        float f = 0.f;
-        if (mine < p.parts) {
-            const float lk = ml[(mine * p.rows + R) * 2 + 1];
-            f = lk != 0.f ? __builtin_amdgcn_exp2f(ml[(mine * p.rows + R) * 2] - m) : 0.f;
-            l += f * lk;
-        }
-        const int count = min(32, (p.parts - k0 + GROUPS - 1) / GROUPS);
-#pragma unroll 8
-        for (int j = 0; j < count; ++j) {
-            const float fj = __shfl(f, (lane & 32) + j);
-            const v4f o = *(const v4f *)(parts + ((long)(k0 + j * GROUPS) * p.rows + R) * p.d4 + d0);
+    float m = -FLT_MAX, l = 0.f;
+    v4f x = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = grp; k0 < p.parts; k0 += BATCH * GROUPS) {
+        v4f o[BATCH];
+        const int first = __builtin_amdgcn_readfirstlane(k0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] += fj != 0.f ? fj * o[i] : 0.f;       // (an empty part was not written)
+        for (int j = 0; j < BATCH; ++j) {                // (one behind the last part: the last one again, with weight zero)
+            o[j] = v4f{0.f, 0.f, 0.f, 0.f};
+            if (first + j * GROUPS < p.parts) o[j] = *(const v4f *)(parts + ((long)min(k0 + j * GROUPS, p.parts - 1) * p.rows + R) * p.d4 + d0);
+        }
+        const int mine = k0 + (q % BATCH) * GROUPS;      // lane q: part q of the batch
+        const float *at = ml + ((long)min(mine, p.parts - 1) * p.rows + R) * 2;
+        const float mk = at[0], lk = mine < p.parts ? at[1] : 0.f;
+        float mn = lk != 0.f ? mk : -FLT_MAX;
+#pragma unroll
+        for (int d = BATCH / 2; d > 0; d >>= 1) mn = fmaxf(mn, __shfl_xor(mn, d));
+        mn = fmaxf(mn, m);
+        const float keep = __builtin_amdgcn_exp2f(m - mn), f = lk != 0.f ? __builtin_amdgcn_exp2f(mk - mn) : 0.f;
+        float lb = f * lk;
+#pragma unroll
+        for (int d = BATCH / 2; d > 0; d >>= 1) lb += __shfl_xor(lb, d);
+        m = mn;
+        l = l * keep + lb;
+        x *= keep;
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            const float fj = __shfl(f, (lane & 32) + j);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] += fj != 0.f ? fj * o[j][i] : 0.f;       // (an empty part was not written)
         }
     }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor(l, d);
+    // the groups' results
     if (BLOCK) {
         sums[grp][q] = x;
-        if (q == 0) ls[grp] = l;
+        if (q == 0) {
+            ls[grp] = l;
+            ms[grp] = m;
+        }
         __syncthreads();
         if (threadIdx.x >= 32) return;
-        for (int g = 1; g < 8; ++g) {
-            x += sums[g][q];
-            l += ls[g];
+        for (int g = 0; g < 8; ++g) m = fmaxf(m, ms[g]);
+        l = 0.f;
+        x = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int g = 0; g < 8; ++g) {
+            const float f = __builtin_amdgcn_exp2f(ms[g] - m);
+            x += f * sums[g][q];
+            l += f * ls[g];
         }
     } else {
-        l += __shfl_xor(l, 32);
+        const float mo = __shfl_xor(m, 32), lo = __shfl_xor(l, 32), mn = fmaxf(m, mo);
+        const float f = __builtin_amdgcn_exp2f(m - mn), fo = __builtin_amdgcn_exp2f(mo - mn);
+        l = f * l + fo * lo;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] += __shfl_xor(x[i], 32);
+        for (int i = 0; i < 4; ++i) x[i] = f * x[i] + fo * __shfl_xor(x[i], 32);
+        m = mn;
         if (lane >= 32) return;
     }
     const int group = a.Hq / a.Hkv, per_seq = a.Lq * group;
@@ -712,9 +720,15 @@ static int attn_go(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
     hipLaunchKernelGGL(kernel, dim3(p.blocks_pre + p.blocks_suf), dim3(256), lds, st, a, p);
     int rc = check_launch();
     if (rc == HPMN_OK && p.parts > 1) {
-        // a workgroup per row while that makes up to eight a CU or the parts are many
-        if (p.rows <= 2048 || p.parts > 32) hipLaunchKernelGGL((prefix_attn_join_kernel<T, true>), dim3((unsigned)p.rows), dim3(256), 0, st, a, p);
-        else hipLaunchKernelGGL((prefix_attn_join_kernel<T, false>), dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0, st, a, p);
+        // a workgroup per row while that makes up to eight a CU or the parts are many; batches that the parts fill (16 where 4 would
+        // do: 1600 rows of 19 parts 5.8 -> 7.4 us; 4 where 16 do: 64 rows of 128 parts 4.6 -> 8.9)
+        if (p.rows <= 2048 || p.parts > 64) {
+            const dim3 grid((unsigned)p.rows);
+            if (p.parts > 32) hipLaunchKernelGGL((prefix_attn_join_kernel<T, true, 16>), grid, dim3(256), 0, st, a, p);
+            else hipLaunchKernelGGL((prefix_attn_join_kernel<T, true, 4>), grid, dim3(256), 0, st, a, p);
+        } else {
+            hipLaunchKernelGGL((prefix_attn_join_kernel<T, false, 8>), dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0, st, a, p);
+        }
         rc = check_launch();
     }
     return rc;
