@@ -16,7 +16,8 @@
 //
 // Rounding choices: scores, maxima, sums and outputs are fp32; the probabilities are rounded to the 16-bit type once, as operand of
 // the second product (half a step each, independent, so about one more rounding of the result).  fp16 probabilities are scaled by
-// 2^15: unscaled, everything below 2^-24 of the largest would vanish, which for long prefixes is most of them.
+// 2^12 (2^15 at most where the maximum lags): unscaled, everything below 2^-24 of the largest would vanish, which for long prefixes
+// is most of them; scaled, what is below 2^-26 of it starts to lose digits and 2^-36 vanishes.
 #pragma once
 #include <algorithm>
 #include <cfloat>
@@ -301,8 +302,9 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int KW = 4 / MW, SUB = attn_sub(sizeof(T), MW), KT = attn_tile(sizeof(T), MW);
     constexpr int EPC = 16 / sizeof(T), CPR = DP / EPC, LD = KT * CPR / 256, DT = DP / 32;
-    constexpr float OFF = std::is_same<T, f16_t>::value ? 15.f : 0.f;
-    constexpr float LAZY = OFF > 0.f ? 0.f : 8.f;       // the maximum may lag by 2^LAZY before O is rescaled
+    constexpr bool F16 = std::is_same<T, f16_t>::value;
+    // probabilities are taken times 2^OFF, and the maximum may lag by 2^LAZY before the output is rescaled: fp16's largest, 2^15, is met
+    constexpr float OFF = F16 ? 12.f : 0.f, LAZY = F16 ? 3.f : 8.f;
     typedef typename Frag<T>::type frag;
     constexpr int BUF = 2 * KT * DP * (int)sizeof(T);    // K and V of a tile; two of them
     char *Kt = lds, *Vt = lds + BUF / 2;
