@@ -99,33 +99,48 @@ struct AttnKeys {
 };
 
 // Tiles from global memory to LDS without passing registers: instruction i of wave w fills the 64 chunk slots from i * 256 + w * 64 on,
-// slot by slot, so a lane picks the chunk that belongs into its slot.  Columns behind D repeat column 0 (their Q is zero, their V is
-// not stored).  Row strides below 2^24 elements: a tile's lane offsets fit 32 bits.
+// slot by slot, so a lane picks the chunk that belongs into its slot.  Lanes of columns behind D load nothing: clear_columns() has put
+// zeros there (their Q is zero too, but 0 * what lies there could be NaN).  Row strides below 2^24 elements: a tile's lane offsets
+// fit 32 bits.
 template <typename T, int DP, int KT>
 struct TileLoader {
     static constexpr int EPC = 16 / sizeof(T), CPR = DP / EPC, LD = KT * CPR / 256, ROWS = 256 / CPR;
     static constexpr int ALT = ROWS < 16 ? 2 : 1;            // the permutation goes by the low four row bits: every other instruction's
     int row, col[ALT], w;
+    bool wide;                               // every column is there (D == DP)
+    bool on[ALT];
     unsigned k_off[ALT], v_off[ALT];
     __device__ __forceinline__ TileLoader(const HpmnPrefixAttn &a, const AttnKeys &src) {
         w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int slot = threadIdx.x;
         row = slot / CPR;
+        wide = a.D == DP;
 #pragma unroll
         for (int j = 0; j < ALT; ++j) {
             col[j] = (chunk_at<CPR>(row + j * ROWS, slot % CPR) - (row + j * ROWS) * CPR) * EPC;
-            if (col[j] >= a.D) col[j] = 0;
+            on[j] = col[j] < a.D;
             k_off[j] = (unsigned)(row * src.kst + col[j]) * (unsigned)sizeof(T);
             v_off[j] = (unsigned)(row * src.vst + col[j]) * (unsigned)sizeof(T);
         }
+    }
+    // zeros into the first `bytes` of the LDS, before the first tile
+    __device__ __forceinline__ void clear_columns(char *lds, int bytes) const {
+        if (wide) return;
+        attn_barrier();                      // (the LDS may be in use by the code in front)
+        for (int i = threadIdx.x; i < bytes / 16; i += 256) *(u32x4 *)(lds + 16 * i) = u32x4{0, 0, 0, 0};
+        attn_barrier();
     }
     // rows k0 .. k0 + KT of `from` (all of them there)
     __device__ __forceinline__ void whole(unsigned lds, const void *from, int64_t stride, const unsigned (&lane_off)[ALT], int k0) const {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             const T *base = (const T *)from + (k0 + i * ROWS) * stride;
-            const unsigned at = lds + i * 4096 + w * 1024;
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(lane_off[i % ALT]), "s"(base) : "memory", "m0");
+            const unsigned at = __builtin_amdgcn_readfirstlane(lds + i * 4096 + w * 1024);
+            if (wide) {
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(lane_off[i % ALT]), "s"(base) : "memory", "m0");
+            } else if (on[i % ALT]) {
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(lane_off[i % ALT]), "s"(base) : "memory", "m0");
+            }
         }
     }
     // rows behind `end` repeat the last one
@@ -133,8 +148,8 @@ struct TileLoader {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             const T *at_row = (const T *)from + min(k0 + row + i * ROWS, end - 1) * stride + col[i % ALT];
-            const unsigned at = lds + i * 4096 + w * 1024;
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(at_row) : "memory", "m0");
+            const unsigned at = __builtin_amdgcn_readfirstlane(lds + i * 4096 + w * 1024);
+            if (on[i % ALT]) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(at_row) : "memory", "m0");
         }
     }
     __device__ __forceinline__ void load(unsigned lds, const void *from, int64_t stride, const unsigned (&lane_off)[ALT], int k0, int end) const {
@@ -269,7 +284,7 @@ __device__ __forceinline__ void attend_whole_tiles(const HpmnPrefixAttn &a, char
         }
         settle_output(scale_out);
     };
-    attn_barrier();                                          // (the LDS may be in use by the code in front)
+    loader.clear_columns(lds, 4 * BUF);
     load_k(0);
     load_v(0);
     load_k(1);
@@ -401,8 +416,9 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
     };
     int buf = 0;
     if (start < src.end) {
-        attn_barrier();                                      // (the LDS may be in use by the code in front)
         if constexpr (VEC) {
+            attn_barrier();                                  // (the LDS may be in use by the code in front)
+            loader.clear_columns(lds, 2 * BUF);
             load(start, 0);
         } else {
             fetch(start);

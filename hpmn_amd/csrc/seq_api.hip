@@ -28,10 +28,11 @@ static inline int prefix_attn_sizes(const HpmnPrefixAttn &a) {
     return HPMN_OK;
 }
 
-// Row strides of the scan: 32 bits (offsets are products of 32-bit numbers in 64 bits).
-static inline bool row_strides_ok(std::initializer_list<int64_t> s) {
+// Row strides of the scan: 32 bits (offsets are products of 32-bit numbers in 64 bits); steps: their number plus a tile in 31.
+static inline bool scan_rows_ok(int T, std::initializer_list<int64_t> s) {
+    if (T > (1 << 30)) return false;
     for (int64_t x : s)
-        if (x >= (1l << 31)) return false;
+        if (T > 1 && x >= (1l << 31)) return false;
     return true;
 }
 
@@ -56,7 +57,7 @@ int hpmn_gated_scan_fwd(const HpmnGatedScan *a, void *stream) {
     if (!a->z || !a->v || !(a->y || a->h_last || a->saved)) return HPMN_EINVAL;
     if (!aligned_to(a->z, a->dtype) || !aligned_to(a->v, a->dtype) || !aligned_to(a->y, a->dtype)) return HPMN_EINVAL;
     if (a->z_sb < 0 || a->z_st < 0 || a->v_sb < 0 || a->v_st < 0 || a->h0_sb < 0 || a->y_sb < 0 || a->y_st < 0) return HPMN_EINVAL;
-    if (!scan_grid_ok(a->B, a->C) || !row_strides_ok({a->z_st, a->v_st, a->y_st})) return HPMN_EUNSUPPORTED;
+    if (!scan_grid_ok(a->B, a->C) || !scan_rows_ok(a->T, {a->z_st, a->v_st, a->y_st})) return HPMN_EUNSUPPORTED;
     const size_t need = gated_scan_workspace_bytes(a->B, a->T, a->C);
     if (need > 0 && (!a->workspace || a->workspace_bytes < need || !is_aligned(a->workspace, 16))) return HPMN_EINVAL;
     return gated_scan_fwd_launch(*a, (hipStream_t)stream);
@@ -74,7 +75,7 @@ int hpmn_gated_scan_bwd(const HpmnGatedScanBwd *a, void *stream) {
     if (a->z_sb < 0 || a->z_st < 0 || a->v_sb < 0 || a->v_st < 0 || a->dy_sb < 0 || a->dy_st < 0 || a->dz_sb < 0 || a->dz_st < 0 ||
         a->dv_sb < 0 || a->dv_st < 0)
         return HPMN_EINVAL;
-    if (!scan_grid_ok(a->B, a->C) || !row_strides_ok({a->z_st, a->v_st, a->dy_st, a->dz_st, a->dv_st})) return HPMN_EUNSUPPORTED;
+    if (!scan_grid_ok(a->B, a->C) || !scan_rows_ok(a->T, {a->z_st, a->v_st, a->dy_st, a->dz_st, a->dv_st})) return HPMN_EUNSUPPORTED;
     const size_t need = gated_scan_workspace_bytes(a->B, a->T, a->C);
     if (need > 0 && (!a->workspace || a->workspace_bytes < need || !is_aligned(a->workspace, 16))) return HPMN_EINVAL;
     return gated_scan_bwd_launch(*a, (hipStream_t)stream);

@@ -53,7 +53,7 @@ def _scan_args(cls):
 
 
 @pytest.mark.parametrize("field,value,rc", [("B", -1, -1), ("T", 0, -1), ("C", 0, -1), ("period", 0, -1), ("period", 3, -1), ("dtype", 3, -1),
-                                            ("z", None, -1), ("v", None, -1), ("z", 4098, -1), ("z_st", -4, -1), ("B", 2 ** 30, -2), ("v_st", 2 ** 31, -2),
+                                            ("z", None, -1), ("v", None, -1), ("z", 4098, -1), ("z_st", -4, -1), ("B", 2 ** 30, -2), ("v_st", 2 ** 31, -2), ("T", 2 ** 30 + 2, -2),
                                             ("B", 0, 0)])
 def test_scan_refusals(lib, field, value, rc):
     for cls, fn in ((_lib.HpmnGatedScan, lib.hpmn_gated_scan_fwd), (_lib.HpmnGatedScanBwd, lib.hpmn_gated_scan_bwd)):

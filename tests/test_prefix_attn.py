@@ -191,6 +191,22 @@ def test_keys_behind_the_lengths_are_not_looked_at(dtype, fill):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("B", [3, 80])
+def test_infinite_keys_beside_unused_columns(dtype, B):
+    """A key of -inf scores takes no part (its score is -inf), also where the kernel pads the head dimension (40 of 64)."""
+    q, kp, vp, _, _ = inputs(B, 1, 1, 1, 40, 300, 0, DTYPES[dtype])
+    q = q.abs()
+    keep = torch.arange(300, device="cuda") % 7 != 3
+    want = check(q, kp[keep].contiguous(), vp[keep].contiguous())
+    kp[~keep] = -float("inf")
+    out, lse = ops.shared_prefix_attention(q, kp, vp, want_lse=True)
+    # the same sums in another order and, for 16-bit types, probabilities of another running maximum: one rounding each
+    assert (out.double() - want[0].double()).abs().max() <= 4 * max(torch.finfo(DTYPES[dtype]).eps, 1e-5)
+    assert (lse - want[1]).abs().max() < 1e-4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
 def test_extreme_scores(dtype):
     """Scores far apart and huge alike: one key takes all; equal keys share; a late key overtakes by a lot.  Many small
     probabilities beside one large one still add up (they would vanish below half a step of the type if they were rounded
@@ -260,10 +276,10 @@ def test_wrapper_refusals():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,Lq", [(4, 1), (200, 1), (3, 20)])
-def test_other_stream_and_captured_graph(B, Lq):
+@pytest.mark.parametrize("B,Lq,D,dtype", [(4, 1, 64, "bf16"), (200, 1, 64, "bf16"), (3, 20, 64, "bf16"), (90, 1, 128, "fp16"), (5, 1, 128, "fp32")])
+def test_other_stream_and_captured_graph(B, Lq, D, dtype):
     """The same numbers on a side stream; a replayed graph follows its inputs, its prefix length and its suffix lengths."""
-    q, kp, vp, ks, vs = inputs(B, Lq, 4, 2, 64, 900, 30, torch.bfloat16)
+    q, kp, vp, ks, vs = inputs(B, Lq, 4, 2, D, 900, 30, DTYPES[dtype])
     plen, slen = i32(900), torch.full((B,), 30, dtype=torch.int32).cuda()
     f = lambda: ops.shared_prefix_attention(q, kp, vp, ks, vs, prefix_len=plen, suffix_len=slen, want_lse=True)  # noqa: E731
     want = f()
