@@ -1,0 +1,113 @@
+"""The sequence operators together, as a layer is trained and a user's candidates are ranked with them."""
+import numpy as np
+import pytest
+import torch
+
+from hpmn_amd import ops
+from test_dropout import oracle_mask
+
+
+def _training_inputs(B, T, D, Cc, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    return r(B, T, D).cuda(), (r(D, 2 * Cc) / D ** 0.5).cuda(), r(B, T // 2, Cc).cuda(), r(B, Cc).cuda()
+
+
+def _layer(x, w, Cc, wy, wh, begin, rng):
+    """One gated linear layer: projection, dropout on the candidates, recurrence that hands on every second state; and back."""
+    B, T, _ = x.shape
+    proj = (x.reshape(B * T, -1) @ w).reshape(B, T, 2 * Cc)
+    z, v = proj[..., :Cc], proj[..., Cc:]
+    dropped = ops.dropout_fwd(v, 0.75, 0, rng=rng)
+    y, h, saved = ops.gated_scan_fwd(z, dropped, begin=begin, period=2, train=True)
+    d_proj = torch.empty_like(proj)
+    _, d_dropped, _ = ops.gated_scan_bwd(z, dropped, saved, wy, d_h_last=wh, begin=begin, period=2, out=(d_proj[..., :Cc], torch.empty_like(dropped)))
+    d_proj[..., Cc:] = ops.dropout_bwd(d_dropped, 0.75, 0, rng=rng)
+    d_w = x.reshape(B * T, -1).t() @ d_proj.reshape(B * T, -1)
+    return y, h, d_w
+
+
+def _layer_float64(x, w, Cc, wy, wh, begin, seed, offset):
+    x, w = x.double().cpu(), w.double().cpu().requires_grad_(True)
+    B, T, _ = x.shape
+    proj = x @ w
+    z, v = proj[..., :Cc], proj[..., Cc:]
+    v = v * torch.from_numpy(oracle_mask(B * T * Cc, 0.75, seed, offset)).reshape(B, T, Cc)
+    h, ys = torch.zeros(B, Cc, dtype=torch.float64), []
+    for t in range(T):
+        a = torch.sigmoid(z[:, t])
+        h = torch.where((begin.cpu() <= t)[:, None], a * h + (1 - a) * v[:, t], h)
+        if t % 2 == 1:
+            ys.append(h)
+    y = torch.stack(ys, 1)
+    ((y * wy.double().cpu()).sum() + (h * wh.double().cpu()).sum()).backward()
+    return y.detach(), h.detach(), w.grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,T,D,Cc", [(3, 40, 16, 24), (5, 300, 32, 64)])
+def test_a_layer_trains(B, T, D, Cc):
+    """States and the weight gradient against float64 autograd: fp32 chains of T steps and sums over B T rows (|terms| of order one,
+    so 2^-24 sqrt(B T) T-independent: 1e-4 of the largest entry covers both products' 2^-24 D and 2^-24 B T)."""
+    x, w, wy, wh = _training_inputs(B, T, D, Cc)
+    begin = torch.tensor([0, T] + [T // 3] * (B - 2), dtype=torch.int32).cuda()
+    rng = torch.tensor([77, 5], device="cuda")
+    got = _layer(x, w, Cc, wy, wh, begin, rng)
+    want = _layer_float64(x, w, Cc, wy, wh, begin, 77, 5)
+    for g, e in zip(got, want):
+        assert (g.double().cpu() - e).abs().max() <= 1e-4 * max(1.0, float(e.abs().max()))
+
+
+@pytest.mark.gpu
+def test_a_captured_layer_draws_and_learns_anew():
+    """The whole step in a graph: replays after eager calls and a new offset give what eager calls give."""
+    x, w, wy, wh = _training_inputs(4, 64, 16, 32)
+    begin = torch.zeros(4, dtype=torch.int32).cuda()
+    rng = torch.tensor([7, 0], device="cuda")
+    _layer(x, w, 32, wy, wh, begin, rng)                               # (the library product's own workspace exists before the capture)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = _layer(x, w, 32, wy, wh, begin, rng)
+    seen = []
+    for k in range(3):
+        rng[1] = 10000 * k
+        x.copy_(_training_inputs(4, 64, 16, 32, seed=k)[0])
+        want = _layer(x, w, 32, wy, wh, begin, rng)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(held, want)), k
+        seen.append(held[2].clone())
+    assert not torch.equal(seen[0], seen[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,N", [(37, 5), (1000, 150)])
+def test_candidates_are_ranked_against_one_history(T, N):
+    """A user's states in bf16 (the scan's y) are the shared prefix; every candidate event is scored as if it came next (a step that
+    is not committed), attends to the history and to itself; then one of them is committed."""
+    H, D = 4, 32
+    Cc = H * D
+    g = torch.Generator().manual_seed(T)
+    z, v = (1 + torch.randn(1, T, Cc, generator=g)).bfloat16().cuda(), torch.randn(1, T, Cc, generator=g).bfloat16().cuda()
+    zc, vc = torch.randn(N, Cc, generator=g).bfloat16().cuda(), torch.randn(N, Cc, generator=g).bfloat16().cuda()
+    y, store, _ = ops.gated_scan_fwd(z, v)
+    user = torch.zeros(N, dtype=torch.int32).cuda()
+    own = ops.gated_scan_step(zc, vc, store, user, commit=False)
+    q = zc.reshape(N, 1, H, D)
+    keys = y[0].reshape(T, H, D)
+    out = ops.shared_prefix_attention(q, keys, keys, own.reshape(N, 1, H, D), own.reshape(N, 1, H, D))
+    # float64, from the operators' own bf16 states (their accuracy is tested where they are)
+    f = lambda t: t.double().cpu()  # noqa: E731
+    a = torch.sigmoid(f(zc))
+    assert (f(own) - (a * f(store) + (1 - a) * f(vc))).abs().max() < 2.0 ** -8 * 4
+    k = torch.cat([f(keys)[None].expand(N, T, H, D), f(own).reshape(N, 1, H, D)], 1)
+    s = (f(q) * k).sum(-1) / D ** 0.5                                  # [N, T + 1, H]
+    want = (torch.softmax(s, 1)[..., None] * k).sum(1)
+    # storage and probabilities each half a step of bf16 of at most max |state|
+    assert (f(out)[:, 0] - want).abs().max() < 2 * 2.0 ** -9 * float(k.abs().max()) + 1e-4
+    before = store.clone()
+    y1 = ops.gated_scan_step(zc[:1], vc[:1], store, user[:1])
+    assert torch.equal(y1, own[:1]) and not torch.equal(store, before)
+    z2, v2 = torch.cat([z, zc[None, :1]], 1), torch.cat([v, vc[None, :1]], 1)
+    assert (ops.gated_scan_fwd(z2, v2)[1] - store).abs().max() < 1e-5
