@@ -1579,10 +1579,17 @@ _SEQ_DTYPES = {torch.float32: _lib.HPMN_F32, torch.bfloat16: _lib.HPMN_BF16, tor
 
 def _chk_seq(name, t, shape, dtype, device):
     """A device tensor of the given shape / dtype whose last dimension is dense (the others may be strided)."""
+    if t.dtype is dtype and t.shape == shape and t.device == device and (t.stride(-1) == 1 or shape[-1] < 2):
+        return
     if t.dtype is not dtype or t.device != device or t.shape != shape:
         raise ValueError("%s: expected %s %s on %s, got %s %s on %s" % (name, tuple(shape), dtype, device, tuple(t.shape), t.dtype, t.device))
-    if shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError("%s: the last dimension has to be dense, got strides %s" % (name, t.stride()))
+    raise ValueError("%s: the last dimension has to be dense, got strides %s" % (name, t.stride()))
+
+
+def _chk_index(name, t, n, device, dtypes=(torch.int32,)):
+    if not (t.dtype in dtypes and t.shape == (n,) and t.device == device and t.is_contiguous()):
+        raise ValueError("%s: expected contiguous %s [%d] on %s, got %s %s on %s"
+                         % (name, " or ".join(str(d)[6:] for d in dtypes), n, device, t.dtype, tuple(t.shape), t.device))
 
 
 def _chk_out(name, t):
@@ -1593,10 +1600,14 @@ def _chk_out(name, t):
 
 
 def _seq_input(name, t, ndim):
-    if t.dim() != ndim or not t.is_cuda or t.dtype not in _SEQ_DTYPES:
+    """The element type's code of the operand that sets shape, type and device of a call; its last dimension is dense."""
+    code = _SEQ_DTYPES.get(t.dtype)
+    if code is None or t.dim() != ndim or not t.is_cuda:
         raise ValueError("%s: expected a %d-dimensional float32 / bfloat16 / float16 CUDA tensor, got %s %s on %s"
                          % (name, ndim, tuple(t.shape), t.dtype, t.device))
-    return _SEQ_DTYPES[t.dtype]
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError("%s: the last dimension has to be dense, got strides %s" % (name, t.stride()))
+    return code
 
 
 # (the raw handle in 0.1 us where building a Stream object takes 2: these calls are a few us in all)
@@ -1615,16 +1626,14 @@ def _call_on(device, name, fn, a):
 
 
 def _gated_scan_shape(z, v, begin, period):
-    _seq_input("z", z, 3)
-    B, T, Cc = z.shape
-    _chk_seq("z", z, z.shape, z.dtype, z.device)
-    _chk_seq("v", v, z.shape, z.dtype, z.device)
+    code, shape, dev = _seq_input("z", z, 3), z.shape, z.device
+    _chk_seq("v", v, shape, z.dtype, dev)
+    B, T, Cc = shape
     if begin is not None:
-        if not (begin.device == z.device and begin.dtype == torch.int32 and tuple(begin.shape) == (B,) and begin.is_contiguous()):
-            raise ValueError("begin: expected contiguous int32 [%d] on %s, got %s %s" % (B, z.device, begin.dtype, tuple(begin.shape)))
+        _chk_index("begin", begin, B, dev)
     if period < 1 or T % period != 0:
         raise ValueError("length %d not divisible by period %d" % (T, period))
-    return B, T, Cc
+    return B, T, Cc, code, dev
 
 
 def _gated_scan_workspace(B, T, Cc, device):
@@ -1642,8 +1651,7 @@ def gated_scan_fwd(z, v, *, h0=None, begin=None, period=1, train=False):
     the state as it is and z, v are not looked at there.  ``period``: every period-th state is handed on (code/hpmn.py:124-128).
     Returns (y [B, T/period, C] in z's dtype, h_last [B, C] float32, saved): ``saved`` is what ``gated_scan_bwd`` needs (None
     unless ``train``)."""
-    B, T, Cc = _gated_scan_shape(z, v, begin, period)
-    dev = z.device
+    B, T, Cc, code, dev = _gated_scan_shape(z, v, begin, period)
     if h0 is not None:
         _chk_seq("h0", h0, (B, Cc), torch.float32, dev)
     y = torch.empty(B, T // period, Cc, device=dev, dtype=z.dtype)
@@ -1659,7 +1667,7 @@ def gated_scan_fwd(z, v, *, h0=None, begin=None, period=1, train=False):
             h_last.copy_(h0)
         return y, h_last, saved
     ws, n = _gated_scan_workspace(B, T, Cc, dev)
-    a = _lib.HpmnGatedScan(B, T, Cc, _SEQ_DTYPES[z.dtype], period, 0, z.data_ptr(), v.data_ptr(), z.stride(0), z.stride(1), v.stride(0),
+    a = _lib.HpmnGatedScan(B, T, Cc, code, period, 0, z.data_ptr(), v.data_ptr(), z.stride(0), z.stride(1), v.stride(0),
                            v.stride(1), _ptr(begin), _ptr(h0), 0 if h0 is None else h0.stride(0), y.data_ptr(), T // period * Cc, Cc,
                            h_last.data_ptr(), _ptr(saved), _ptr(ws), n)
     _call_on(dev, "hpmn_gated_scan_fwd", _lib.load().hpmn_gated_scan_fwd, a)
@@ -1670,8 +1678,7 @@ def gated_scan_bwd(z, v, saved, d_y, *, d_h_last=None, begin=None, period=1, out
     """hpmn_gated_scan_bwd: gradients of ``gated_scan_fwd`` (same ``z``, ``v``, ``begin``, ``period``; ``saved`` from its training
     form).  ``d_y`` [B, T/period, C] in z's dtype or None, ``d_h_last`` [B, C] float32 or None.  ``out`` = (d_z, d_v): buffers to
     write into, e.g. the halves of one projection's gradient (strided).  Returns (d_z, d_v, d_h0 float32 [B, C])."""
-    B, T, Cc = _gated_scan_shape(z, v, begin, period)
-    dev = z.device
+    B, T, Cc, code, dev = _gated_scan_shape(z, v, begin, period)
     tiles = -(-T // _lib.HPMN_GATED_SCAN_TILE)
     if saved is None:
         raise ValueError("saved: gated_scan_fwd has to run with train=True")
@@ -1702,7 +1709,7 @@ def gated_scan_bwd(z, v, saved, d_y, *, d_h_last=None, begin=None, period=1, out
         return d_z, d_v, d_h0
     ws, n = _gated_scan_workspace(B, T, Cc, dev)
     dy_sb, dy_st = (0, 0) if d_y is None else (d_y.stride(0), d_y.stride(1))
-    a = _lib.HpmnGatedScanBwd(B, T, Cc, _SEQ_DTYPES[z.dtype], period, 0, z.data_ptr(), v.data_ptr(), z.stride(0), z.stride(1),
+    a = _lib.HpmnGatedScanBwd(B, T, Cc, code, period, 0, z.data_ptr(), v.data_ptr(), z.stride(0), z.stride(1),
                               v.stride(0), v.stride(1), _ptr(begin), saved.data_ptr(), _ptr(d_y), dy_sb, dy_st, _ptr(d_h_last),
                               d_z.data_ptr(), d_v.data_ptr(), d_z.stride(0), d_z.stride(1), d_v.stride(0), d_v.stride(1),
                               d_h0.data_ptr(), _ptr(ws), n)
@@ -1718,27 +1725,26 @@ def gated_scan_step(z, v, state, user=None, *, commit=True):
     ``commit``: the new states are written to the store; events of the same user are applied in row order.  Without it the store
     is only read (a candidate event scored as if it were the next one; any user may be named any number of times).  A row whose
     user is outside the store changes nothing and gets NaN."""
-    _seq_input("z", z, 2)
-    B, Cc = z.shape
-    dev = z.device
-    _chk_seq("z", z, z.shape, z.dtype, dev)
-    _chk_seq("v", v, z.shape, z.dtype, dev)
+    code, shape, dev = _seq_input("z", z, 2), z.shape, z.device
+    B, Cc = shape
+    _chk_seq("v", v, shape, z.dtype, dev)
     if state.dim() != 2:
         raise ValueError("state: expected [n_users, %d], got %s" % (Cc, tuple(state.shape)))
-    _chk_seq("state", state, (state.shape[0], Cc), torch.float32, dev)
-    _chk_out("state", state)
-    if user is None:
-        if state.shape[0] != B:
-            raise ValueError("%d rows against %d states: pass user" % (B, state.shape[0]))
-    elif not (user.device == dev and user.dtype in (torch.int32, torch.int64) and tuple(user.shape) == (B,) and user.is_contiguous()):
-        raise ValueError("user: expected contiguous int32 or int64 [%d] on %s, got %s %s" % (B, dev, user.dtype, tuple(user.shape)))
+    users, state_s = state.shape[0], state.stride(0)
+    _chk_seq("state", state, (users, Cc), torch.float32, dev)
+    if state_s < Cc and users > 1:
+        raise ValueError("state: overlapping rows, strides %s" % (state.stride(),))
+    if user is not None:
+        _chk_index("user", user, B, dev, (torch.int32, torch.int64))
+    elif users != B:
+        raise ValueError("%d rows against %d states: pass user" % (B, users))
     y = torch.empty(B, Cc, device=dev, dtype=z.dtype)
-    if y.numel() == 0:
+    if B == 0 or Cc == 0:
         return y
     flags = (_lib.HPMN_STEP_COMMIT if commit else 0) | (_lib.HPMN_STEP_USER_I64 if user is not None and user.dtype is torch.int64 else 0)
     zs, vs = z.stride(0), v.stride(0)
-    a = _lib.HpmnGatedStep(B, Cc, _SEQ_DTYPES[z.dtype], flags, z.data_ptr(), v.data_ptr(), zs, vs, state.data_ptr(),
-                           max(state.stride(0), Cc), state.shape[0], _ptr(user), y.data_ptr(), Cc)
+    a = _lib.HpmnGatedStep(B, Cc, code, flags, z.data_ptr(), v.data_ptr(), zs, vs, state.data_ptr(), max(state_s, Cc), users, _ptr(user),
+                           y.data_ptr(), Cc)
     fn = _lib.load().hpmn_gated_scan_step
     # the ordered form works through its user list in calls of HPMN_STEP_MAX_INDEXED rows (one stream: still in row order)
     most = _lib.HPMN_STEP_MAX_INDEXED
@@ -1764,24 +1770,26 @@ def _as_rows(t, Cc):
 
 
 def _dropout(name, x, keep_prob, seed, offset, residual, rng):
-    if x.dim() == 0:
-        raise ValueError("%s: a tensor of at least one dimension" % name)
-    _seq_input("x", x, x.dim())
+    code, dev, shape = _SEQ_DTYPES.get(x.dtype), x.device, x.shape
+    if code is None or not x.is_cuda or len(shape) == 0:
+        raise ValueError("%s: expected a float32 / bfloat16 / float16 CUDA tensor of at least one dimension, got %s %s on %s"
+                         % (name, tuple(shape), x.dtype, dev))
     if not 0.0 < keep_prob <= 1.0:
         raise ValueError("keep_prob has to be in (0, 1], got %r" % (keep_prob,))
-    dev, shape = x.device, x.shape
-    if rng is not None and not (rng.device == dev and rng.dtype == torch.int64 and tuple(rng.shape) == (2,) and rng.is_contiguous()):
-        raise ValueError("rng: expected contiguous int64 [2] on %s" % dev)
-    if residual is not None:
-        _chk_seq("residual", residual, shape, x.dtype, dev)
+    if rng is not None:
+        _chk_index("rng", rng, 2, dev, (torch.int64,))
+    if residual is not None and not (residual.dtype is x.dtype and residual.shape == shape and residual.device == dev):
+        raise ValueError("residual: expected %s %s on %s, got %s %s on %s"
+                         % (tuple(shape), x.dtype, dev, tuple(residual.shape), residual.dtype, residual.device))
     y = torch.empty(shape, device=dev, dtype=x.dtype)
-    if y.numel() == 0:
+    n = x.numel()
+    if n == 0:
         return y
     Cc = shape[-1]
     x, x_s = _as_rows(x, Cc)
     if residual is not None:
         residual, r_s = _as_rows(residual, Cc)
-    a = _lib.HpmnDropout(y.numel() // Cc, Cc, _SEQ_DTYPES[x.dtype], keep_prob, x.data_ptr(), _ptr(residual), y.data_ptr(), x_s,
+    a = _lib.HpmnDropout(n // Cc, Cc, code, keep_prob, x.data_ptr(), _ptr(residual), y.data_ptr(), x_s,
                          0 if residual is None else r_s, Cc, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _ptr(rng))
     _call_on(dev, "hpmn_dropout", _lib.load().hpmn_dropout, a)
     return y
@@ -1812,10 +1820,8 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k_suffix=None, v_suffix=None,
     ``prefix_len``: int32 [1] on the device, the prefix in use (None: P).  ``suffix_len``: int32 [B] (None: S); with several query
     tokens they are the last of the suffix and see it up to their own position.  ``scale``: default D ** -0.5.  Returns out
     [B, Lq, Hq, D] (a query without any key: zeros), with ``want_lse`` also the log-sum-exp [B, Lq, Hq] float32 (-inf there)."""
-    dt = _seq_input("q", q, 4)
+    dt, dev = _seq_input("q", q, 4), q.device
     B, Lq, Hq, D = q.shape
-    dev = q.device
-    _chk_seq("q", q, q.shape, q.dtype, dev)
     if k_prefix.dim() != 3:
         raise ValueError("k_prefix: expected [P, Hkv, D], got %s" % (tuple(k_prefix.shape),))
     P, Hkv = k_prefix.shape[:2]
@@ -1834,16 +1840,17 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k_suffix=None, v_suffix=None,
         S = k_suffix.shape[1]
         _chk_seq("k_suffix", k_suffix, (B, S, Hkv, D), q.dtype, dev)
         _chk_seq("v_suffix", v_suffix, (B, S, Hkv, D), q.dtype, dev)
-    for name, t, n in (("prefix_len", prefix_len, 1), ("suffix_len", suffix_len, B)):
-        if t is not None and not (t.device == dev and t.dtype == torch.int32 and tuple(t.shape) == (n,) and t.is_contiguous()):
-            raise ValueError("%s: expected contiguous int32 [%d] on %s, got %s %s" % (name, n, dev, t.dtype, tuple(t.shape)))
+    if prefix_len is not None:
+        _chk_index("prefix_len", prefix_len, 1, dev)
+    if suffix_len is not None:
+        _chk_index("suffix_len", suffix_len, B, dev)
     if scale is None:
         scale = D ** -0.5
     if not math.isfinite(scale):
         raise ValueError("scale has to be finite, got %r" % (scale,))
     out = torch.empty(B, Lq, Hq, D, device=dev, dtype=q.dtype)
     lse = torch.empty(B, Lq, Hq, device=dev, dtype=torch.float32) if want_lse else None
-    if out.numel() > 0:
+    if B > 0 and Lq > 0:
         ks = (k_suffix.data_ptr(), v_suffix.data_ptr()) if S else (None, None)
         kst, vst = (k_suffix.stride()[:3], v_suffix.stride()[:3]) if S else ((0, 0, 0), (0, 0, 0))
         a = _lib.HpmnPrefixAttn(B, Lq, Hq, Hkv, D, dt, P, S, scale, 0, q.data_ptr(), *q.stride()[:3], k_prefix.data_ptr(),
