@@ -2,7 +2,7 @@
 // instantiates it: prefix_attn.hip, prefix_attn_bf16.hip, prefix_attn_f16.hip).
 //
 // The query rows of one key head -- every (sequence, query token, grouped head) -- are a matrix of M = B Lq Hq / Hkv rows against the
-// SAME prefix, so the prefix is a matrix product's operand: a workgroup takes 128 rows (or 64 or 32, when there are few) and a range of
+// SAME prefix, so the prefix is a matrix product's operand: a workgroup takes 128 rows (or 64, when there are few) and a range of
 // keys, and K and V are read once per 128 rows instead of once per row.  One pass with the running maximum and sum:
 //   S^T = K Q^T   a wave: 32 query rows (columns of S^T: one row per lane pair, so maximum and sum are a register reduction and ONE
 //                 exchange between the wave's halves), 32 keys at a time on the matrix pipe, Q in registers throughout;
@@ -10,7 +10,7 @@
 //                 the keys, and V is read in that order (16-bit: transposing LDS reads, four keys x 16 columns per 16 lanes).
 // K and V tiles go from global memory to LDS directly, the next tile in flight while this one is used; LDS chunks of 16 bytes are
 // permuted by the row number so that neither the reads along a row nor those across sixteen rows meet in a bank.
-// Few rows: two or all four waves of a workgroup share out the keys of a tile and join their results in LDS.  The key
+// Few rows: the waves of a workgroup share out the keys of a tile two by two and join their results in LDS.  The key
 // axis is split over workgroups until the chip is full; a second kernel joins the parts (maximum, sum, unnormalised output in fp32).
 // A row's own suffix is the same thing with M = Lq Hq / Hkv rows and a key limit per row, in the same launch.
 //
@@ -755,8 +755,6 @@ static int attn_go(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
 template <typename T, int DP, bool VEC>
 static int attn_rows(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
     if (p.mw_pre == 4) return p.mw_suf == 4 ? attn_go<T, DP, VEC, 4, 4>(a, p, st) : attn_go<T, DP, VEC, 4, 2>(a, p, st);
-    if constexpr (sizeof(T) == 2)
-        if (p.mw_pre == 1) return attn_go<T, DP, VEC, 1, 2>(a, p, st);
     return attn_go<T, DP, VEC, 2, 2>(a, p, st);
 }
 

@@ -7,30 +7,39 @@ namespace hpmn {
 extern template int prefix_attn_type<bf16_t>(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st);
 extern template int prefix_attn_type<f16_t>(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st);
 
-// By sizes and type alone.  Rows: 128 per workgroup from 65 on (below, the waves share out keys; four ways only for 16-bit types,
-// whose tiles leave room for it: 8 x 8 heads over 1 of 64, 32768 keys 16.3 us against 21.3 two ways).  Keys: split until about two
-// workgroups per CU exist.
+// By sizes and type alone.  Rows: 128 per workgroup from 65 on, 64 below (two waves share out the keys; four waves for up to 32 rows,
+// 16-bit: 8 rows of 64 over 32768 keys 11.9 against 12.1 us, 4 x 32 heads over 8 of 128 29.1 against 29.7: not kept).
 AttnPlan attn_plan(const HpmnPrefixAttn &a) {
     AttnPlan p = {};
     const int esize = (int)elem_size(a.dtype), group = a.Hq / a.Hkv;
     const long M = (long)a.B * a.Lq * group, per_seq = (long)a.Lq * group;
     p.rows = M * a.Hkv;
     p.d4 = (a.D + 3) / 4 * 4;
-    p.mw_pre = M > 64 ? 4 : M > 32 || esize == 4 ? 2 : 1;
+    p.mw_pre = M > 64 ? 4 : 2;
     p.mw_suf = per_seq > 64 ? 4 : 2;
     auto split = [&](long base, int keys, int tile, int &splits, int &per) {
         const int tiles = std::max(1, (keys + tile - 1) / tile);
-        // one workgroup per CU, two when each still has 1280 keys (fp32: 320) to work through (a tile's loads hide behind the other's products;
-        // shorter ranges pay more for their start and for the join): 300 x 8 heads of 128, 16384 keys 54 -> 50 us with two,
-        // 200 x 8 heads over 2 of 64, 4096 keys 17.5 -> 21 us
+        // Keys: one workgroup per CU, two when each still has 1280 keys (fp32: 320) to work through -- a tile's loads hide behind the
+        // other's products, shorter ranges pay more for their start and for the join: 300 x 8 heads of 128, 16384 keys 54 -> 50 us with
+        // two, 200 x 8 heads over 2 of 64, 4096 keys 17.5 -> 21.  At most 128 parts to join (fp32, whose ranges cost more: 256):
+        // 8 x 8 heads over 1 of 64, 32768 keys 13.8 us against 15.3 with 256 and 15.8 with 64; fp32, 8 rows 20.9 against 16.5 with 256.
         splits = (int)std::max<long>(1, std::min<long>(tiles, 256 / base));
         if ((long)tiles * tile / splits >= (esize == 4 ? 320 : 1280)) splits = (int)std::max<long>(1, std::min<long>(tiles, 512 / base));
+        splits = std::min(splits, esize == 4 ? 256 : 128);
         per = (tiles + splits - 1) / splits * tile;
         splits = std::max(1, (keys + per - 1) / per);
     };
+    // a short prefix and nothing else: one range, no second kernel.  8 x 8 heads over 2 of 64, 512 keys bf16: 9.0 us of device time
+    // against 9.1 cut up, and one launch less to wait for; 1024 keys 12.6 against 9.2; 200 x 8 heads over 2 of 64, 256 keys 11.4
+    // against 11.0, over 8 of 128 17.5 against 13.5
+    const bool whole = a.S == 0 && esize == 2 && (long)a.P * a.D <= (p.mw_pre == 4 ? 256 : 512) * 64;
     p.rt_pre = (int)((M + 32 * p.mw_pre - 1) / (32 * p.mw_pre));
     // (16-bit, many rows: pairs of tiles)
     split((long)p.rt_pre * a.Hkv, a.P, attn_tile(esize, p.mw_pre) * (esize == 2 && p.mw_pre == 4 ? 2 : 1), p.splits_pre, p.per_pre);
+    if (whole) {
+        p.splits_pre = 1;
+        p.per_pre = std::max(a.P, 1);
+    }
     p.blocks_pre = (unsigned)(((long)a.Hkv * p.splits_pre + 7) / 8 * 8 * p.rt_pre);
     if (a.S > 0) {
         p.rt_suf = (int)((per_seq + 32 * p.mw_suf - 1) / (32 * p.mw_suf));
