@@ -1696,8 +1696,8 @@ def gated_scan_bwd(z, v, saved, d_y, *, d_h_last=None, begin=None, period=1, out
             _chk_seq(n, t, (B, T, Cc), z.dtype, dev)
             _chk_out(n, t)
     else:
-        d_z = torch.empty(B, T, Cc, device=dev, dtype=z.dtype)
-        d_v = torch.empty(B, T, Cc, device=dev, dtype=z.dtype)
+        d_z = torch.empty_like(z, memory_format=torch.contiguous_format)
+        d_v = torch.empty_like(z, memory_format=torch.contiguous_format)
     d_h0 = torch.empty(B, Cc, device=dev, dtype=torch.float32)
     if d_h0.numel() == 0:
         return d_z, d_v, d_h0
@@ -1738,7 +1738,7 @@ def gated_scan_step(z, v, state, user=None, *, commit=True):
         _chk_index("user", user, B, dev, (torch.int32, torch.int64))
     elif users != B:
         raise ValueError("%d rows against %d states: pass user" % (B, users))
-    y = torch.empty(B, Cc, device=dev, dtype=z.dtype)
+    y = torch.empty_like(z, memory_format=torch.contiguous_format)
     if B == 0 or Cc == 0:
         return y
     flags = (_lib.HPMN_STEP_COMMIT if commit else 0) | (_lib.HPMN_STEP_USER_I64 if user is not None and user.dtype is torch.int64 else 0)
@@ -1781,7 +1781,7 @@ def _dropout(name, x, keep_prob, seed, offset, residual, rng):
     if residual is not None and not (residual.dtype is x.dtype and residual.shape == shape and residual.device == dev):
         raise ValueError("residual: expected %s %s on %s, got %s %s on %s"
                          % (tuple(shape), x.dtype, dev, tuple(residual.shape), residual.dtype, residual.device))
-    y = torch.empty(shape, device=dev, dtype=x.dtype)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     n = x.numel()
     if n == 0:
         return y
@@ -1848,7 +1848,7 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k_suffix=None, v_suffix=None,
         scale = D ** -0.5
     if not math.isfinite(scale):
         raise ValueError("scale has to be finite, got %r" % (scale,))
-    out = torch.empty(B, Lq, Hq, D, device=dev, dtype=q.dtype)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty(B, Lq, Hq, device=dev, dtype=torch.float32) if want_lse else None
     if B > 0 and Lq > 0:
         ks = (k_suffix.data_ptr(), v_suffix.data_ptr()) if S else (None, None)
