@@ -169,11 +169,11 @@ __device__ __forceinline__ void attn_arrive() { asm volatile("s_waitcnt vmcnt(0)
 // needed a tile before V: after the barrier in front of tile k, K(k + 1) and V(k) are there, and the buffers of K(k) and V(k - 1)
 // are free, so two buffers each, one barrier per tile, and a tile's time for the loads.  Tiles go in pairs so that buffers are
 // constants and an LDS address is one of NX + DT registers and an immediate.
-template <typename T, int DP>
+template <typename T, int DP, int DC>
 __device__ __forceinline__ void attend_whole_tiles(const HpmnPrefixAttn &a, char *lds, const AttnKeys &src, int full,
-                                                   const typename Frag<T>::type (&qf)[DP / 16], float c, float off, float lazy,
-                                                   v16f (&o)[DP / 32], float &m, float &l) {
-    constexpr int KT = 64, CPR = DP / 8, NX = DP / 16, DT = DP / 32, BUF = KT * DP * 2;
+                                                   const typename Frag<T>::type (&qf)[DC / 16], float c, float off, float lazy,
+                                                   v16f (&o)[DC / 32], float &m, float &l) {
+    constexpr int KT = 64, CPR = DP / 8, NX = DC / 16, DT = DC / 32, BUF = KT * DP * 2;
     typedef typename Frag<T>::type frag;
     typedef __attribute__((address_space(3))) char lds_char;
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -311,12 +311,12 @@ __device__ __forceinline__ void attend_whole_tiles(const HpmnPrefixAttn &a, char
     }
 }
 
-template <typename T, int DP, bool VEC, int MW>
+template <typename T, int DP, int DC, bool VEC, int MW>
 __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &p, char *lds, const AttnKeys &src, int kvh, int row0,
                                        int row_end) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int KW = 4 / MW, SUB = attn_sub(sizeof(T), MW), KT = attn_tile(sizeof(T), MW);
-    constexpr int EPC = 16 / sizeof(T), CPR = DP / EPC, LD = KT * CPR / 256, DT = DP / 32;
+    constexpr int EPC = 16 / sizeof(T), CPR = DP / EPC, LD = KT * CPR / 256, DT = DC / 32;
     constexpr bool F16 = std::is_same<T, f16_t>::value;
     // probabilities are taken times 2^OFF, and the maximum may lag by 2^LAZY before the output is rescaled: fp16's largest, 2^15, is met
     constexpr float OFF = F16 ? 12.f : 0.f, LAZY = F16 ? 3.f : 8.f;
@@ -334,11 +334,11 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
     const int limit = src.suffix ? min(src.end, max(0, src.seen + tok)) : src.end;
 
     // Q: column `row` of the first product's second operand, d in the order of the chunks this half of the wave reads
-    frag qf[DP / (2 * EPC)];
+    frag qf[DC / (2 * EPC)];
     {
         const T *q = (const T *)a.q + b * a.q_sb + tok * a.q_sl + h * a.q_sh;
 #pragma unroll
-        for (int s = 0; s < DP / (2 * EPC); ++s) {
+        for (int s = 0; s < DC / (2 * EPC); ++s) {
             const int d0 = (2 * s + half) * EPC;
             if constexpr (VEC) {
                 const frag x = *(const frag *)(q + (d0 < a.D ? d0 : 0));
@@ -355,7 +355,7 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
         // a negative scale becomes a sign of q, a zero one a zero q: what multiplies the scores is positive
         if (a.scale <= 0.f) {
 #pragma unroll
-            for (int s = 0; s < DP / (2 * EPC); ++s)
+            for (int s = 0; s < DC / (2 * EPC); ++s)
 #pragma unroll
                 for (int e = 0; e < EPC; ++e) qf[s][e] = a.scale < 0.f ? -qf[s][e] : (T)0.f;
         }
@@ -404,7 +404,7 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
     if constexpr (!F32 && MW == 4 && VEC) {
         const int full = (src.end - src.begin) / (2 * KT) * 2;
         if (!src.suffix && full > 0) {
-            attend_whole_tiles<T, DP>(a, lds, src, full, qf, c, OFF, LAZY, o, m, l);
+            attend_whole_tiles<T, DP, DC>(a, lds, src, full, qf, c, OFF, LAZY, o, m, l);
             start = src.begin + full * KT;
         }
     }
@@ -454,7 +454,7 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
 #pragma unroll
-            for (int x = 0; x < DP / (2 * EPC); ++x) {
+            for (int x = 0; x < DC / (2 * EPC); ++x) {
                 const frag kf = *(const frag *)(Kt + buf + 16 * chunk_at<CPR>(kb + 32 * u + n, 2 * x + half));
                 if constexpr (F32) {
 #pragma unroll
@@ -563,7 +563,7 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
             for (int g = 0; g < 4; ++g)
                 put_quad(row, b, tok, h, 32 * t + 8 * g + 4 * half, v4f{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]}, l);
     } else {
-        constexpr int RS = DP + 4;                       // a row of the join, in floats
+        constexpr int RS = DC + 4;                       // a row of the join, in floats
         float *ob = (float *)lds, *mb = ob + 4 * 32 * RS;
         attn_barrier();
         if (active) {
@@ -578,8 +578,8 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
             }
         }
         attn_barrier();
-        for (int i = tid; i < MW * 32 * (DP / 4); i += 256) {
-            const int jr = i / (DP / 4), d = i % (DP / 4) * 4, rr = row0 + jr;
+        for (int i = tid; i < MW * 32 * (DC / 4); i += 256) {
+            const int jr = i / (DC / 4), d = i % (DC / 4) * 4, rr = row0 + jr;
             if (rr >= row_end) break;
             float mm = -FLT_MAX, ll = 0.f;
 #pragma unroll
@@ -599,8 +599,8 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
     }
 }
 
-template <typename T, int DP, bool VEC, int MWP, int MWS>
-__global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128) ? 1 : 2) void prefix_attn_kernel(const HpmnPrefixAttn a, const AttnPlan p) {
+template <typename T, int DP, int DC, bool VEC, int MWP, int MWS>
+__global__ __launch_bounds__(256, (sizeof(T) == 4 && (DC == 128 || (DC == 96 && !VEC))) ? 1 : 2) void prefix_attn_kernel(const HpmnPrefixAttn a, const AttnPlan p) {
     extern __shared__ char attn_smem[];
     const int group = a.Hq / a.Hkv;
     AttnKeys k;
@@ -620,7 +620,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128) ? 1 : 2) void pr
         k.part = split;
         k.suffix = false;
         k.b = k.seen = 0;
-        attend<T, DP, VEC, MWP>(a, p, attn_smem, k, kvh, rt * 32 * MWP, a.B * a.Lq * group);
+        attend<T, DP, DC, VEC, MWP>(a, p, attn_smem, k, kvh, rt * 32 * MWP, a.B * a.Lq * group);
     } else {
         unsigned j = blockIdx.x - p.blocks_pre;
         const int rt = j % p.rt_suf;
@@ -639,7 +639,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128) ? 1 : 2) void pr
         k.suffix = true;
         k.b = b;
         k.seen = len - a.Lq + 1;
-        attend<T, DP, VEC, MWS>(a, p, attn_smem, k, kvh, rt * 32 * MWS, a.Lq * group);
+        attend<T, DP, DC, VEC, MWS>(a, p, attn_smem, k, kvh, rt * 32 * MWS, a.Lq * group);
     }
 }
 
@@ -724,10 +724,10 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(const HpmnPrefixA
     if (a.lse && q == 0) a.lse[((long)b * a.Lq + tok) * a.Hq + h] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
-template <typename T, int DP, bool VEC, int MWP, int MWS>
+template <typename T, int DP, int DC, bool VEC, int MWP, int MWS>
 static int attn_go(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
     const size_t lds = std::max(attn_lds(sizeof(T), DP, MWP), attn_lds(sizeof(T), DP, MWS));
-    auto kernel = prefix_attn_kernel<T, DP, VEC, MWP, MWS>;
+    auto kernel = prefix_attn_kernel<T, DP, DC, VEC, MWP, MWS>;
     if (lds > 64 * 1024) {
         hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) {
@@ -752,17 +752,20 @@ static int attn_go(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
     return rc;
 }
 
-template <typename T, int DP, bool VEC>
+template <typename T, int DP, int DC, bool VEC>
 static int attn_rows(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
-    if (p.mw_pre == 4) return p.mw_suf == 4 ? attn_go<T, DP, VEC, 4, 4>(a, p, st) : attn_go<T, DP, VEC, 4, 2>(a, p, st);
-    return attn_go<T, DP, VEC, 2, 2>(a, p, st);
+    if (p.mw_pre == 4) return p.mw_suf == 4 ? attn_go<T, DP, DC, VEC, 4, 4>(a, p, st) : attn_go<T, DP, DC, VEC, 4, 2>(a, p, st);
+    return attn_go<T, DP, DC, VEC, 2, 2>(a, p, st);
 }
 
+// Columns: LDS rows of 32, 64 or 128, of which 96 are multiplied for D in 65 .. 96 (fewer registers, so fp32 has two
+// waves a SIMD: 158 x 16 heads over 8 of 96, 7850 keys 145 -> 115 us; bf16, 512 x 16 heads over 4 of 96, 8192 keys 60.2 -> 54.1).
 template <typename T>
 static int attn_width(const HpmnPrefixAttn &a, const AttnPlan &p, bool vec, hipStream_t st) {
-    if (a.D <= 32) return vec ? attn_rows<T, 32, true>(a, p, st) : attn_rows<T, 32, false>(a, p, st);
-    if (a.D <= 64) return vec ? attn_rows<T, 64, true>(a, p, st) : attn_rows<T, 64, false>(a, p, st);
-    return vec ? attn_rows<T, 128, true>(a, p, st) : attn_rows<T, 128, false>(a, p, st);
+    if (a.D <= 32) return vec ? attn_rows<T, 32, 32, true>(a, p, st) : attn_rows<T, 32, 32, false>(a, p, st);
+    if (a.D <= 64) return vec ? attn_rows<T, 64, 64, true>(a, p, st) : attn_rows<T, 64, 64, false>(a, p, st);
+    if (a.D <= 96) return vec ? attn_rows<T, 128, 96, true>(a, p, st) : attn_rows<T, 128, 96, false>(a, p, st);
+    return vec ? attn_rows<T, 128, 128, true>(a, p, st) : attn_rows<T, 128, 128, false>(a, p, st);
 }
 
 template <typename T>
