@@ -27,11 +27,17 @@
 
 namespace hpmn {
 
+constexpr int JOIN_KEYS = 8;                 // at most so many suffix keys are the second kernel's
+
 struct AttnPlan {
     int mw_pre, mw_suf;                      // waves along the rows (the other 4 / mw along the keys)
     int rt_pre, rt_suf;                      // row tiles per key head / per sequence and key head
     int splits_pre, splits_suf, per_pre, per_suf;   // key ranges and their length
-    int parts;                               // splits_pre + splits_suf; 1: no second kernel, results go straight out
+    int parts;                               // splits_pre + splits_suf
+    int keys;                                // suffix keys that the second kernel takes itself (then there are no suffix ranges)
+    bool join;                               // a second kernel; else results go straight out
+    bool vec;                                // 16-byte accesses: whole 16 bytes in a row, aligned pointers and strides
+    bool out_vec;                            // outputs four columns at a time
     int d4;                                  // D rounded up to 4: a row of a part
     long rows;                               // Hkv * M
     long o_at;                               // where the parts' outputs start in the workspace, in floats (behind their m and l)
@@ -39,7 +45,7 @@ struct AttnPlan {
 };
 
 AttnPlan attn_plan(const HpmnPrefixAttn &a);
-template <typename T> int prefix_attn_type(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st);
+template <typename T> int prefix_attn_type(const HpmnPrefixAttn &a, AttnPlan &p, hipStream_t st);
 
 // Keys per tile and LDS bytes of a configuration.
 constexpr int attn_sub(int esize, int mw) { return esize == 2 && mw == 4 ? 2 : 1; }
@@ -533,7 +539,7 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
     float *ml = (float *)a.workspace, *parts = ml + p.o_at;
     const long M = p.rows / a.Hkv;
     auto put_ml = [&](int rr, int bb, int tt, int hh, float mm, float ll) {
-        if (p.parts > 1) {
+        if (p.join) {
             float *at = ml + (src.part * p.rows + kvh * M + (src.suffix ? (long)bb * per_seq : 0) + rr) * 2;
             at[0] = mm;
             at[1] = ll;
@@ -543,20 +549,19 @@ __device__ __forceinline__ void attend(const HpmnPrefixAttn &a, const AttnPlan &
     };
     auto put_quad = [&](int rr, int bb, int tt, int hh, int d, v4f x, float ll) {
         if (d >= a.D) return;
-        if (p.parts > 1) {
+        if (p.join) {
             *(v4f *)(parts + (src.part * p.rows + kvh * M + (src.suffix ? (long)bb * per_seq : 0) + rr) * p.d4 + d) = x;
         } else {
             const float inv = ll == 0.f ? 0.f : 1.0f / ll;
             T *out = (T *)a.out + bb * a.o_sb + tt * a.o_sl + hh * a.o_sh + d;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (d + i < a.D) out[i] = (T)(x[i] * inv);
+            if (p.out_vec) store_quad<T, true>(out, x * inv, 4);
+            else store_quad<T, false>(out, x * inv, a.D - d);
         }
     };
     if constexpr (KW == 1) {
         if (row >= row_end) return;
         if (half == 0) put_ml(row, b, tok, h, m, l);
-        if (l == 0.f && p.parts > 1) return;             // (nothing was seen: the second kernel does not look)
+        if (l == 0.f && p.join) return;             // (nothing was seen: the second kernel does not look)
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -646,7 +651,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && (DC == 128 || (DC == 96 && 
 // Second kernel: joins a row's parts.  Groups of 32 lanes (a quad of the row each, D <= 128) take the parts in turn, BATCH at a
 // time; BLOCK: a workgroup of eight groups per row, else a wave of two.  What the parts hold was written by other XCDs, a round trip to
 // memory is most of this kernel: a batch's outputs are asked for before its weights are known, and both in one go.
-template <typename T, bool BLOCK, int BATCH>
+// OWN > 0: the few keys of a short suffix are parts too, of one key each (the score is the maximum, the value the output), OWN to a group,
+// grp, grp + GROUPS ...; VEC: their rows and q's in aligned quads.
+template <typename T, bool BLOCK, int BATCH, int OWN, bool VEC>
 __global__ __launch_bounds__(256) void prefix_attn_join_kernel(const HpmnPrefixAttn a, const AttnPlan p) {
     constexpr int GROUPS = BLOCK ? 8 : 2;
     __shared__ v4f sums[8][32];
@@ -656,8 +663,23 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(const HpmnPrefixA
     const int lane = threadIdx.x & 63, q = lane & 31, grp = BLOCK ? (int)threadIdx.x >> 5 : lane >> 5;
     const float *ml = (const float *)a.workspace, *parts = ml + p.o_at;
     const int d0 = min(4 * q, p.d4 - 4);
+    const int group = a.Hq / a.Hkv, per_seq = a.Lq * group;
+    const long M = p.rows / a.Hkv;
+    const int kvh = (int)(R / M), r = (int)(R % M), b = r / per_seq, tok = r % per_seq / group, h = kvh * group + r % group;
     float m = -FLT_MAX, l = 0.f;
     v4f x = {0.f, 0.f, 0.f, 0.f};
+    quad_t<T> qf, kf[OWN ? OWN : 1], vf[OWN ? OWN : 1];
+    if constexpr (OWN > 0) {                             // asked for before the parts; what is not to be seen is loaded and not used
+        const T *Q = (const T *)a.q + b * a.q_sb + tok * a.q_sl + h * a.q_sh;
+        const T *K = (const T *)a.k_suf + b * a.ks_sb + kvh * a.ks_sh, *V = (const T *)a.v_suf + b * a.vs_sb + kvh * a.vs_sh;
+        qf = load_quad<T, VEC>(Q + d0, a.D - d0);        // (d0 < D; columns behind D: anything)
+#pragma unroll
+        for (int j = 0; j < OWN; ++j) {
+            const int key = min(grp + j * GROUPS, a.S - 1);
+            kf[j] = load_quad<T, VEC>(K + key * a.ks_st + d0, a.D - d0);
+            vf[j] = load_quad<T, VEC>(V + key * a.vs_st + d0, a.D - d0);
+        }
+    }
     for (int k0 = grp; k0 < p.parts; k0 += BATCH * GROUPS) {
         v4f o[BATCH];
         const int first = __builtin_amdgcn_readfirstlane(k0);
@@ -687,6 +709,36 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(const HpmnPrefixA
             for (int i = 0; i < 4; ++i) x[i] += fj != 0.f ? fj * o[j][i] : 0.f;       // (an empty part was not written)
         }
     }
+    if constexpr (OWN > 0) {
+        const int len = a.suffix_len ? min(max(a.suffix_len[b], 0), a.S) : a.S, limit = min(len, len - a.Lq + 1 + tok);
+        const float c = a.scale == 0.f ? 1.f : -NEG_LOG2E * fabsf(a.scale);
+        float sc[OWN], mn = m;
+#pragma unroll
+        for (int j = 0; j < OWN; ++j) {
+            sc[j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e = a.scale == 0.f ? 0.f : a.scale < 0.f ? -(float)qf[i] : (float)qf[i];
+                sc[j] = 4 * q + i < a.D ? fmaf(e, (float)kf[j][i], sc[j]) : sc[j];
+            }
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) sc[j] += __shfl_xor(sc[j], d);
+            sc[j] *= c;
+            if (grp + j * GROUPS < limit) mn = fmaxf(mn, sc[j]);
+        }
+        const float keep = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= keep;
+        x *= keep;
+#pragma unroll
+        for (int j = 0; j < OWN; ++j) {
+            if (grp + j * GROUPS >= limit) break;
+            const float f = __builtin_amdgcn_exp2f(sc[j] - mn);
+            l += f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = fmaf(f, (float)vf[j][i], x[i]);
+        }
+    }
     // the groups' results
     if (BLOCK) {
         sums[grp][q] = x;
@@ -713,15 +765,20 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(const HpmnPrefixA
         m = mn;
         if (lane >= 32) return;
     }
-    const int group = a.Hq / a.Hkv, per_seq = a.Lq * group;
-    const long M = p.rows / a.Hkv;
-    const int kvh = (int)(R / M), r = (int)(R % M), b = r / per_seq, tok = r % per_seq / group, h = kvh * group + r % group;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     T *out = (T *)a.out + b * a.o_sb + tok * a.o_sl + h * a.o_sh + 4 * q;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (4 * q + i < a.D) out[i] = (T)(x[i] * inv);
+    if (4 * q < a.D) {
+        if (p.out_vec) store_quad<T, true>(out, x * inv, 4);
+        else store_quad<T, false>(out, x * inv, a.D - 4 * q);
+    }
     if (a.lse && q == 0) a.lse[((long)b * a.Lq + tok) * a.Hq + h] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+template <typename T, bool BLOCK, int BATCH, int OWN, bool VEC>
+static void attn_join(const HpmnPrefixAttn &a, const AttnPlan &p, long blocks, hipStream_t st) {
+    const dim3 grid((unsigned)blocks);
+    if (p.keys > 0) hipLaunchKernelGGL((prefix_attn_join_kernel<T, BLOCK, BATCH, OWN, VEC>), grid, dim3(256), 0, st, a, p);
+    else hipLaunchKernelGGL((prefix_attn_join_kernel<T, BLOCK, BATCH, 0, true>), grid, dim3(256), 0, st, a, p);
 }
 
 template <typename T, int DP, int DC, bool VEC, int MWP, int MWS>
@@ -737,15 +794,17 @@ static int attn_go(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
     }
     hipLaunchKernelGGL(kernel, dim3(p.blocks_pre + p.blocks_suf), dim3(256), lds, st, a, p);
     int rc = check_launch();
-    if (rc == HPMN_OK && p.parts > 1) {
+    if (rc == HPMN_OK && p.join) {
+        const int parts = p.parts + p.keys;
         // a workgroup per row while that makes up to eight a CU or the parts are many; batches that the parts fill (16 where 4 would
         // do: 1600 rows of 19 parts 5.8 -> 7.4 us; 4 where 16 do: 64 rows of 128 parts 4.6 -> 8.9)
-        if (p.rows <= 2048 || p.parts > 64) {
-            const dim3 grid((unsigned)p.rows);
-            if (p.parts > 32) hipLaunchKernelGGL((prefix_attn_join_kernel<T, true, 16>), grid, dim3(256), 0, st, a, p);
-            else hipLaunchKernelGGL((prefix_attn_join_kernel<T, true, 4>), grid, dim3(256), 0, st, a, p);
+        if (p.rows <= 2048 || parts > 64) {
+            if (p.parts > 32) attn_join<T, true, 16, 1, VEC>(a, p, p.rows, st);
+            else attn_join<T, true, 4, 1, VEC>(a, p, p.rows, st);
+        } else if (p.keys <= 2) {
+            attn_join<T, false, 8, 1, VEC>(a, p, (p.rows + 3) / 4, st);
         } else {
-            hipLaunchKernelGGL((prefix_attn_join_kernel<T, false, 8>), dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0, st, a, p);
+            attn_join<T, false, 8, JOIN_KEYS / 2, VEC>(a, p, (p.rows + 3) / 4, st);
         }
         rc = check_launch();
     }
@@ -761,23 +820,24 @@ static int attn_rows(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st)
 // Columns: LDS rows of 32, 64 or 128, of which 96 are multiplied for D in 65 .. 96 (fewer registers, so fp32 has two
 // waves a SIMD: 158 x 16 heads over 8 of 96, 7850 keys 145 -> 115 us; bf16, 512 x 16 heads over 4 of 96, 8192 keys 60.2 -> 54.1).
 template <typename T>
-static int attn_width(const HpmnPrefixAttn &a, const AttnPlan &p, bool vec, hipStream_t st) {
-    if (a.D <= 32) return vec ? attn_rows<T, 32, 32, true>(a, p, st) : attn_rows<T, 32, 32, false>(a, p, st);
-    if (a.D <= 64) return vec ? attn_rows<T, 64, 64, true>(a, p, st) : attn_rows<T, 64, 64, false>(a, p, st);
-    if (a.D <= 96) return vec ? attn_rows<T, 128, 96, true>(a, p, st) : attn_rows<T, 128, 96, false>(a, p, st);
-    return vec ? attn_rows<T, 128, 128, true>(a, p, st) : attn_rows<T, 128, 128, false>(a, p, st);
+static int attn_width(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
+    if (a.D <= 32) return p.vec ? attn_rows<T, 32, 32, true>(a, p, st) : attn_rows<T, 32, 32, false>(a, p, st);
+    if (a.D <= 64) return p.vec ? attn_rows<T, 64, 64, true>(a, p, st) : attn_rows<T, 64, 64, false>(a, p, st);
+    if (a.D <= 96) return p.vec ? attn_rows<T, 128, 96, true>(a, p, st) : attn_rows<T, 128, 96, false>(a, p, st);
+    return p.vec ? attn_rows<T, 128, 128, true>(a, p, st) : attn_rows<T, 128, 128, false>(a, p, st);
 }
 
 template <typename T>
-int prefix_attn_type(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st) {
+int prefix_attn_type(const HpmnPrefixAttn &a, AttnPlan &p, hipStream_t st) {
     constexpr int E = 16 / sizeof(T);
-    bool vec = a.D % E == 0;
-    for (const void *q : {a.q, a.k_pre, a.v_pre, a.k_suf, a.v_suf}) vec = vec && is_aligned(q, 16);
+    p.vec = a.D % E == 0;
+    for (const void *q : {a.q, a.k_pre, a.v_pre, a.k_suf, a.v_suf}) p.vec = p.vec && is_aligned(q, 16);
     for (int64_t s : {a.q_sb, a.q_sl, a.q_sh, a.kp_st, a.kp_sh, a.vp_st, a.vp_sh, a.ks_sb, a.ks_st, a.ks_sh, a.vs_sb, a.vs_st, a.vs_sh})
-        vec = vec && s % E == 0;
-    for (int64_t s : {a.kp_st, a.vp_st, a.ks_st, a.vs_st}) vec = vec && s < (1l << 24);      // TileLoader: 128 rows in 32 bits of bytes
-    return attn_width<T>(a, p, vec, st);
+        p.vec = p.vec && s % E == 0;
+    for (int64_t s : {a.kp_st, a.vp_st, a.ks_st, a.vs_st}) p.vec = p.vec && s < (1l << 24);  // TileLoader: 128 rows in 32 bits of bytes
+    p.out_vec = a.D % 4 == 0 && is_aligned(a.out, 4 * sizeof(T));
+    for (int64_t s : {a.o_sb, a.o_sl, a.o_sh}) p.out_vec = p.out_vec && s % 4 == 0;
+    return attn_width<T>(a, p, st);
 }
-
 
 }  // namespace hpmn

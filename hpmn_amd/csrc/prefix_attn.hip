@@ -4,8 +4,8 @@
 
 namespace hpmn {
 
-extern template int prefix_attn_type<bf16_t>(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st);
-extern template int prefix_attn_type<f16_t>(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st);
+extern template int prefix_attn_type<bf16_t>(const HpmnPrefixAttn &a, AttnPlan &p, hipStream_t st);
+extern template int prefix_attn_type<f16_t>(const HpmnPrefixAttn &a, AttnPlan &p, hipStream_t st);
 
 // By sizes and type alone.  Rows: 128 per workgroup from 65 on, 64 below (two waves share out the keys; four waves for up to 32 rows,
 // 16-bit: 8 rows of 64 over 32768 keys 11.9 against 12.1 us, 4 x 32 heads over 8 of 128 29.1 against 29.7: not kept).
@@ -44,21 +44,30 @@ AttnPlan attn_plan(const HpmnPrefixAttn &a) {
     if (a.S > 0) {
         p.rt_suf = (int)((per_seq + 32 * p.mw_suf - 1) / (32 * p.mw_suf));
         const long base = (long)a.B * a.Hkv * p.rt_suf;
-        split(base, a.S, attn_tile(esize, p.mw_suf), p.splits_suf, p.per_suf);
-        p.blocks_suf = (unsigned)(base * p.splits_suf);
+        // Few keys of very many sequences: the second kernel's, which asks for them beside the parts.  A workgroup for each costs its
+        // start and its own part: 300 x 8 heads of 128 over 4096 keys + 1 45.6 -> 27.6 us, 1000 x 16 heads over 2 of 128, 2048 + 8
+        // 75.0 -> 62.8, 64 x 8 heads of 128, 4096 + 1 22.6 -> 18.8; up to 512 of them run beside the prefix's (500 x 1 head of 64,
+        // 1000 + 1 11.3 against 11.7, 8 x 8 heads over 1 of 64 12.1 against 12.7).
+        if (a.S <= JOIN_KEYS && base >= 512) {
+            p.keys = a.S;
+        } else {
+            split(base, a.S, attn_tile(esize, p.mw_suf), p.splits_suf, p.per_suf);
+            p.blocks_suf = (unsigned)(base * p.splits_suf);
+        }
     }
     p.parts = p.splits_pre + p.splits_suf;
+    p.join = p.parts > 1 || p.keys > 0;
     p.o_at = ((long)p.parts * p.rows * 2 + 3) / 4 * 4;
     return p;
 }
 
 size_t prefix_attn_workspace_bytes(const HpmnPrefixAttn &a) {
     const AttnPlan p = attn_plan(a);
-    return p.parts > 1 ? ((size_t)p.o_at + (size_t)p.parts * p.rows * p.d4) * sizeof(float) : 0;
+    return p.join ? ((size_t)p.o_at + (size_t)p.parts * p.rows * p.d4) * sizeof(float) : 0;
 }
 
 int prefix_attn_launch(const HpmnPrefixAttn &a, hipStream_t st) {
-    const AttnPlan p = attn_plan(a);
+    AttnPlan p = attn_plan(a);
     if (a.dtype == HPMN_F32) return prefix_attn_type<float>(a, p, st);
     return a.dtype == HPMN_BF16 ? prefix_attn_type<bf16_t>(a, p, st) : prefix_attn_type<f16_t>(a, p, st);
 }

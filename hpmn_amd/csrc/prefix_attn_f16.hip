@@ -3,6 +3,6 @@
 
 namespace hpmn {
 
-template int prefix_attn_type<f16_t>(const HpmnPrefixAttn &a, const AttnPlan &p, hipStream_t st);
+template int prefix_attn_type<f16_t>(const HpmnPrefixAttn &a, AttnPlan &p, hipStream_t st);
 
 }  // namespace hpmn

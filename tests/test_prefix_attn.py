@@ -153,6 +153,50 @@ def test_against_float64(size, dtype):
     check(*x, plen=i32(max(0, P - 3)), scale=-0.3 / D ** 0.5)
 
 
+MANY = [  # a few own keys of very many sequences: joined with the prefix's parts
+    (600, 1, 1, 1, 64, 100, 1), (130, 3, 8, 4, 96, 300, 3), (256, 2, 4, 2, 40, 70, 8), (512, 1, 2, 1, 17, 40, 5), (512, 1, 1, 1, 32, 2100, 4),
+    (1100, 1, 2, 1, 128, 200, 2), (1030, 1, 4, 1, 24, 90, 7), (2100, 1, 1, 1, 3, 0, 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("size", MANY)
+def test_few_keys_of_many_sequences(size, dtype):
+    B, Lq, Hq, Hkv, D, P, S = size
+    q, kp, vp, ks, vs = inputs(*size, DTYPES[dtype], seed=sum(size))
+    check(q, kp, vp, ks, vs)
+    n = torch.randint(-1, S + 2, (B,), generator=torch.Generator().manual_seed(2), dtype=torch.int32)
+    want = check(q, kp, vp, ks, vs, slen=n.cuda(), scale=-0.4 / D ** 0.5)
+    for b in range(B):
+        for t in (ks, vs):
+            t[b, max(0, int(n[b])):] = float("nan")
+    got = ops.shared_prefix_attention(q, kp, vp, ks, vs, suffix_len=n.cuda(), scale=-0.4 / D ** 0.5, want_lse=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_few_keys_of_many_sequences_strides(dtype):
+    """Head-major storage, one key row for all, odd storage offsets, no scale, a prefix of length zero."""
+    dt = DTYPES[dtype]
+    q, kp, vp, ks, vs = inputs(300, 1, 4, 2, 64, 150, 4, dt)
+    want = check(q, kp, vp, ks, vs)
+    major = lambda t: t.transpose(-2, -3).contiguous().transpose(-2, -3)  # noqa: E731
+    assert torch.equal(check(q, kp, vp, major(ks), major(vs))[0], want[0])
+    flat = torch.empty(2, ks.numel() + 1, device="cuda", dtype=dt)
+    ko, vo = flat[0, 1:].view(ks.shape), flat[1, :-1].view(vs.shape)
+    ko.copy_(ks)
+    vo.copy_(vs)
+    check(q, kp, vp, ko, vo)
+    check(q, kp, vp, ks[:, :1].expand(300, 4, 2, 64), vs)
+    check(q, kp, vp, ks, vs, scale=0.0)
+    check(q, kp, vp, ks, vs, plen=i32(0))
+    ks[7] = -float("inf")                                              # scores of -inf where q's sign is one: no part
+    q[7] = q[7].abs()
+    out = ops.shared_prefix_attention(q, kp, vp, ks, vs)
+    assert (out[7].double() - ops.shared_prefix_attention(q[7:8], kp, vp)[0].double()).abs().max() <= 4 * max(torch.finfo(dt).eps, 1e-5)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
 def test_lengths(dtype):
