@@ -663,13 +663,19 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(const HpmnPrefixA
     const int lane = threadIdx.x & 63, q = lane & 31, grp = BLOCK ? (int)threadIdx.x >> 5 : lane >> 5;
     const float *ml = (const float *)a.workspace, *parts = ml + p.o_at;
     const int d0 = min(4 * q, p.d4 - 4);
-    const int group = a.Hq / a.Hkv, per_seq = a.Lq * group;
-    const long M = p.rows / a.Hkv;
-    const int kvh = (int)(R / M), r = (int)(R % M), b = r / per_seq, tok = r % per_seq / group, h = kvh * group + r % group;
+    int kvh, b, tok, h;
+    const auto locate = [&] {                            // the row's place (32-bit divisions: all rows are at most 2^26)
+        const unsigned group = a.Hq / a.Hkv, per_seq = a.Lq * group, M = a.B * per_seq, row = (unsigned)R, r = row % M, is = r % per_seq;
+        kvh = row / M;
+        b = r / per_seq;
+        tok = is / group;
+        h = kvh * group + is % group;
+    };
     float m = -FLT_MAX, l = 0.f;
     v4f x = {0.f, 0.f, 0.f, 0.f};
     quad_t<T> qf, kf[OWN ? OWN : 1], vf[OWN ? OWN : 1];
     if constexpr (OWN > 0) {                             // asked for before the parts; what is not to be seen is loaded and not used
+        locate();
         const T *Q = (const T *)a.q + b * a.q_sb + tok * a.q_sl + h * a.q_sh;
         const T *K = (const T *)a.k_suf + b * a.ks_sb + kvh * a.ks_sh, *V = (const T *)a.v_suf + b * a.vs_sb + kvh * a.vs_sh;
         qf = load_quad<T, VEC>(Q + d0, a.D - d0);        // (d0 < D; columns behind D: anything)
@@ -765,6 +771,7 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(const HpmnPrefixA
         m = mn;
         if (lane >= 32) return;
     }
+    if constexpr (OWN == 0) locate();
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     T *out = (T *)a.out + b * a.o_sb + tok * a.o_sl + h * a.o_sh + 4 * q;
     if (4 * q < a.D) {
