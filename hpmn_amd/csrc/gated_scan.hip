@@ -516,6 +516,14 @@ static Cut scan_cut(int B, int T, int C) {
     return {(tiles + per - 1) / per, per};
 }
 
+// A launch has to stay below 2^32 threads, steps and a tile more in 31 bits.
+bool gated_scan_fits(int B, int T, int C) {
+    if (T > (1 << 30) || C > (1 << 30)) return false;
+    const int lpr = scan_lanes(C);
+    const Cut cut = scan_cut(B, T, C);
+    return (double)B * ((C + 4l * lpr - 1) / (4 * lpr)) * cut.chunks * 64 * scan_waves(T, lpr) < 4294967296.0;
+}
+
 size_t gated_scan_workspace_bytes(int B, int T, int C) {
     const Cut cut = scan_cut(B, T, C);
     return cut.chunks > 1 ? (size_t)B * cut.chunks * 2 * C * sizeof(float) : 0;

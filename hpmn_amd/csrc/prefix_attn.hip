@@ -68,6 +68,8 @@ size_t prefix_attn_workspace_bytes(const HpmnPrefixAttn &a) {
 
 int prefix_attn_launch(const HpmnPrefixAttn &a, hipStream_t st) {
     AttnPlan p = attn_plan(a);
+    // a launch has to stay below 2^32 threads
+    if ((uint64_t)p.blocks_pre + p.blocks_suf >= (1u << 24) || (p.join && (p.rows + 3) / 4 >= (1l << 24))) return HPMN_EUNSUPPORTED;
     if (a.dtype == HPMN_F32) return prefix_attn_type<float>(a, p, st);
     return a.dtype == HPMN_BF16 ? prefix_attn_type<bf16_t>(a, p, st) : prefix_attn_type<f16_t>(a, p, st);
 }

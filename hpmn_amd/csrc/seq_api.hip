@@ -5,6 +5,7 @@
 
 namespace hpmn {
 
+bool gated_scan_fits(int B, int T, int C);
 size_t gated_scan_workspace_bytes(int B, int T, int C);
 int gated_scan_fwd_launch(const HpmnGatedScan &a, hipStream_t st);
 int gated_scan_bwd_launch(const HpmnGatedScanBwd &a, hipStream_t st);
@@ -15,9 +16,6 @@ int dropout_launch(const HpmnDropout &a, unsigned threshold, hipStream_t st);
 
 static inline bool known_dtype(int d) { return d == HPMN_F32 || d == HPMN_BF16 || d == HPMN_F16; }
 static inline bool aligned_to(const void *p, int dtype) { return is_aligned(p, elem_size(dtype)); }
-
-// One grid dimension and 32-bit block indices: (sequences) x (channel blocks) has to stay below 2^31.
-static inline bool scan_grid_ok(int B, int C) { return (long)B * ((C + 15) / 16) < (1l << 30); }
 
 // Sizes that every index of the attention kernels fits: query rows, keys and work items in 31 bits, head groups whole.
 static inline int prefix_attn_sizes(const HpmnPrefixAttn &a) {
@@ -45,7 +43,7 @@ static inline void drop_stale_hip_error() { (void)hipGetLastError(); }
 extern "C" {
 
 size_t hpmn_gated_scan_workspace_bytes(int32_t B, int32_t T, int32_t C) {
-    if (B < 1 || T < 1 || C < 1 || !scan_grid_ok(B, C)) return 0;
+    if (B < 1 || T < 1 || C < 1 || !gated_scan_fits(B, T, C)) return 0;
     return gated_scan_workspace_bytes(B, T, C);
 }
 
@@ -57,7 +55,7 @@ int hpmn_gated_scan_fwd(const HpmnGatedScan *a, void *stream) {
     if (!a->z || !a->v || !(a->y || a->h_last || a->saved)) return HPMN_EINVAL;
     if (!aligned_to(a->z, a->dtype) || !aligned_to(a->v, a->dtype) || !aligned_to(a->y, a->dtype)) return HPMN_EINVAL;
     if (a->z_sb < 0 || a->z_st < 0 || a->v_sb < 0 || a->v_st < 0 || a->h0_sb < 0 || a->y_sb < 0 || a->y_st < 0) return HPMN_EINVAL;
-    if (!scan_grid_ok(a->B, a->C) || !scan_rows_ok(a->T, {a->z_st, a->v_st, a->y_st})) return HPMN_EUNSUPPORTED;
+    if (!gated_scan_fits(a->B, a->T, a->C) || !scan_rows_ok(a->T, {a->z_st, a->v_st, a->y_st})) return HPMN_EUNSUPPORTED;
     const size_t need = gated_scan_workspace_bytes(a->B, a->T, a->C);
     if (need > 0 && (!a->workspace || a->workspace_bytes < need || !is_aligned(a->workspace, 16))) return HPMN_EINVAL;
     return gated_scan_fwd_launch(*a, (hipStream_t)stream);
@@ -75,7 +73,7 @@ int hpmn_gated_scan_bwd(const HpmnGatedScanBwd *a, void *stream) {
     if (a->z_sb < 0 || a->z_st < 0 || a->v_sb < 0 || a->v_st < 0 || a->dy_sb < 0 || a->dy_st < 0 || a->dz_sb < 0 || a->dz_st < 0 ||
         a->dv_sb < 0 || a->dv_st < 0)
         return HPMN_EINVAL;
-    if (!scan_grid_ok(a->B, a->C) || !scan_rows_ok(a->T, {a->z_st, a->v_st, a->dy_st, a->dz_st, a->dv_st})) return HPMN_EUNSUPPORTED;
+    if (!gated_scan_fits(a->B, a->T, a->C) || !scan_rows_ok(a->T, {a->z_st, a->v_st, a->dy_st, a->dz_st, a->dv_st})) return HPMN_EUNSUPPORTED;
     const size_t need = gated_scan_workspace_bytes(a->B, a->T, a->C);
     if (need > 0 && (!a->workspace || a->workspace_bytes < need || !is_aligned(a->workspace, 16))) return HPMN_EINVAL;
     return gated_scan_bwd_launch(*a, (hipStream_t)stream);
@@ -92,7 +90,7 @@ int hpmn_gated_scan_step(const HpmnGatedStep *a, void *stream) {
     if (!aligned_to(a->z, a->dtype) || !aligned_to(a->v, a->dtype) || !aligned_to(a->y, a->dtype)) return HPMN_EINVAL;
     if (a->z_s < 0 || a->v_s < 0 || a->y_s < 0 || a->state_s < a->C) return HPMN_EINVAL;
     if (a->user && (a->flags & HPMN_STEP_COMMIT) && a->B > HPMN_STEP_MAX_INDEXED) return HPMN_EUNSUPPORTED;
-    if ((long)a->B * ((a->C + 3) / 4) >= (1l << 36)) return HPMN_EUNSUPPORTED;
+    if (a->B >= (1 << 26)) return HPMN_EUNSUPPORTED;             // a launch: below 2^32 threads, 64 a row here
     return gated_step_launch(*a, (hipStream_t)stream);
 }
 
@@ -105,7 +103,7 @@ int hpmn_dropout(const HpmnDropout *a, void *stream) {
     if (!aligned_to(a->x, a->dtype) || !aligned_to(a->y, a->dtype) || !aligned_to(a->residual, a->dtype)) return HPMN_EINVAL;
     if (!is_aligned(a->rng, 8)) return HPMN_EINVAL;
     if (a->x_s < 0 || a->r_s < 0 || (a->N > 1 && a->y_s < a->C)) return HPMN_EINVAL;
-    if (a->N > (1l << 40) / a->C) return HPMN_EUNSUPPORTED;      // one launch: 2^30 blocks of at least 1024 elements
+    if (a->N > ((1l << 34) - 1024) / a->C) return HPMN_EUNSUPPORTED;     // a launch: below 2^32 threads, four elements or more each
     // floor(p 2^16 + 1/2), as a double: p is a float, so the product is exact
     const double q = (double)a->keep_prob * 65536.0 + 0.5;
     const unsigned thr = q < 1.0 ? 1u : (unsigned)q;

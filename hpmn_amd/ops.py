@@ -1587,16 +1587,19 @@ def _chk_seq(name, t, shape, dtype, device):
 
 
 def _chk_index(name, t, n, device, dtypes=(torch.int32,)):
-    if not (t.dtype in dtypes and t.shape == (n,) and t.device == device and t.is_contiguous()):
-        raise ValueError("%s: expected contiguous %s [%d] on %s, got %s %s on %s"
-                         % (name, " or ".join(str(d)[6:] for d in dtypes), n, device, t.dtype, tuple(t.shape), t.device))
+    if not (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.shape == (n,) and t.device == device and t.is_contiguous()):
+        raise ValueError("%s: expected contiguous %s [%d] on %s, got %s"
+                         % (name, " or ".join(str(d)[6:] for d in dtypes), n, device,
+                            "%s %s on %s" % (t.dtype, tuple(t.shape), t.device) if isinstance(t, torch.Tensor) else repr(t)))
 
 
 def _chk_out(name, t):
-    """An output's rows must not overlap: every stride in front of the dense last dimension covers a row."""
-    for d in range(t.dim() - 1):
-        if t.shape[d] > 1 and t.stride(d) < t.shape[-1]:
+    """An output's elements must not overlap: by rising stride, every dimension steps over all of those before it."""
+    reach = 1
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if s < reach:
             raise ValueError("%s: overlapping rows, strides %s" % (name, t.stride()))
+        reach += s * (n - 1)
 
 
 def _seq_input(name, t, ndim):
@@ -1677,7 +1680,7 @@ def gated_scan_fwd(z, v, *, h0=None, begin=None, period=1, train=False):
 def gated_scan_bwd(z, v, saved, d_y, *, d_h_last=None, begin=None, period=1, out=None):
     """hpmn_gated_scan_bwd: gradients of ``gated_scan_fwd`` (same ``z``, ``v``, ``begin``, ``period``; ``saved`` from its training
     form).  ``d_y`` [B, T/period, C] in z's dtype or None, ``d_h_last`` [B, C] float32 or None.  ``out`` = (d_z, d_v): buffers to
-    write into, e.g. the halves of one projection's gradient (strided).  Returns (d_z, d_v, d_h0 float32 [B, C])."""
+    write into, e.g. the halves of one projection's gradient (strided), apart from the inputs and each other.  Returns (d_z, d_v, d_h0 float32 [B, C])."""
     B, T, Cc, code, dev = _gated_scan_shape(z, v, begin, period)
     tiles = -(-T // _lib.HPMN_GATED_SCAN_TILE)
     if saved is None:
@@ -1695,6 +1698,8 @@ def gated_scan_bwd(z, v, saved, d_y, *, d_h_last=None, begin=None, period=1, out
         for n, t in (("d_z", d_z), ("d_v", d_v)):
             _chk_seq(n, t, (B, T, Cc), z.dtype, dev)
             _chk_out(n, t)
+        if d_z.data_ptr() == d_v.data_ptr() and d_z.numel() > 0:
+            raise ValueError("out: d_z and d_v are the same memory")
     else:
         d_z = torch.empty_like(z, memory_format=torch.contiguous_format)
         d_v = torch.empty_like(z, memory_format=torch.contiguous_format)

@@ -801,6 +801,8 @@ int hpmn_memory_update(const HpmnOnlineUpdate *args, void *stream);
  * Backward, with G_t = dL/dh_t in full:
  *   G_t = d_y[fires at t] + a_{t+1} G_{t+1}  (+ d_h_last at T-1);   d_v = (1-a) G;   d_z = G (h_{t-1} - v) a (1-a);
  *   d_h0 = a_0 G_0.   Deterministic.  d_z / d_v / d_h0 are overwritten; d_y, d_h_last, d_h0 may be NULL (zero / not wanted).
+ * No output overlaps an input or another output.  Calls of more work than one launch has threads for (2^32; at 512 threads per 64
+ * channels of a sequence of 128 steps or more) are refused with HPMN_EUNSUPPORTED, here and in the calls below.
  * workspace: >= hpmn_gated_scan_workspace_bytes(B, T, C) bytes (16-byte aligned; may be 0 bytes: NULL then), used by this call only.
  * ---------------------------------------------------------------------------------- */
 #define HPMN_F32 0

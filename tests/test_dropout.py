@@ -38,6 +38,13 @@ def test_refusals(lib, field, value, rc):
     assert lib.hpmn_dropout(None, None) == -1
 
 
+@pytest.mark.parametrize("N,Cc", [(1 << 28, 64), (1 << 34, 1), (1, 1 << 34), (1 << 62, 3)])
+def test_more_threads_than_a_launch_has_are_refused(lib, N, Cc):
+    a = _args()
+    a.N, a.C, a.y_s, a.x_s = N, Cc, Cc, Cc
+    assert lib.hpmn_dropout(C.byref(a), None) == -2
+
+
 def test_struct_layout(tmp_path):
     st = _lib.HpmnDropout
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "hpmn_hip.h"', 'int main(void){printf("%zu", sizeof(HpmnDropout));']

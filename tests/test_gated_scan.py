@@ -64,6 +64,18 @@ def test_scan_refusals(lib, field, value, rc):
     assert lib.hpmn_gated_scan_workspace_bytes(0, 8, 8) == 0 and lib.hpmn_gated_scan_workspace_bytes(-1, 8, 8) == 0
 
 
+@pytest.mark.parametrize("B,T,Cc", [(1 << 24, 128, 64), (1 << 26, 1, 16), (1, 2 ** 31 - 1, 1), (1 << 10, 128, 1 << 30), (2 ** 31 - 1, 1, 2 ** 31 - 1)])
+def test_more_threads_than_a_launch_has_are_refused(lib, B, T, Cc):
+    for cls, fn in ((_lib.HpmnGatedScan, lib.hpmn_gated_scan_fwd), (_lib.HpmnGatedScanBwd, lib.hpmn_gated_scan_bwd)):
+        a = _scan_args(cls)
+        a.B, a.T, a.C, a.period = B, T, Cc, 1
+        assert fn(C.byref(a), None) == -2
+    assert lib.hpmn_gated_scan_workspace_bytes(B, T, Cc) == 0
+    s = _lib.HpmnGatedStep()
+    s.B, s.C, s.z, s.v, s.state, s.y, s.z_s, s.v_s, s.y_s, s.state_s, s.n_users = 1 << 26, 4, 4096, 4096, 4096, 4096, 4, 4, 4, 4, 1 << 26
+    assert lib.hpmn_gated_scan_step(C.byref(s), None) == -2
+
+
 def test_scan_needs_an_output_and_saved_states(lib):
     a = _scan_args(_lib.HpmnGatedScan)
     a.y = a.h_last = a.saved = None
@@ -321,7 +333,9 @@ def test_wrapper_refusals():
            lambda: ops.gated_scan_fwd(z, z, begin=torch.zeros(3, device="cuda", dtype=torch.int32)),
            lambda: ops.gated_scan_fwd(z.transpose(1, 2), z.transpose(1, 2)), lambda: ops.gated_scan_fwd(z[0], z[0]),
            lambda: ops.gated_scan_bwd(z, z, None, z), lambda: ops.gated_scan_bwd(z, z, saved[:1], z), lambda: ops.gated_scan_bwd(z, z, saved, z[:, :3]),
-           lambda: ops.gated_scan_bwd(z, z, saved, z, out=(z, z[:, :1].expand(2, 6, 8))), lambda: ops.gated_scan_bwd(z, z, saved, z.half()),
+           lambda: ops.gated_scan_bwd(z, z, saved, z, out=(z, z[:, :1].expand(2, 6, 8))),
+           lambda: ops.gated_scan_bwd(z, z, saved, z, out=(z.clone(), torch.as_strided(z.clone(), (2, 6, 8), (8, 8, 1)))),
+           lambda: ops.gated_scan_bwd(z, z, saved, z, out=(z, z)), lambda: ops.gated_scan_fwd(z, z, begin=[0, 1]), lambda: ops.gated_scan_bwd(z, z, saved, z.half()),
            lambda: ops.gated_scan_step(z[0], z[0], z[0, :5]), lambda: ops.gated_scan_step(z[0], z[0], z[0].half()),
            lambda: ops.gated_scan_step(z[0], z[1], z[0, :1].expand(6, 8)),
            lambda: ops.gated_scan_step(z[0], z[0], z[0], torch.zeros(6, device="cuda")), lambda: ops.gated_scan_step(z, z, z[0])]

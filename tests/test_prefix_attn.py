@@ -51,6 +51,13 @@ def test_workspace_is_asked_for(lib, sizes):
             assert lib.hpmn_prefix_attn(C.byref(a), None) == -1
 
 
+@pytest.mark.parametrize("sizes", [(1 << 25, 1, 1, 1, 8, 16, 16), (1, 1, 1 << 24, 1 << 24, 8, 16, 0), (1 << 26, 1, 1, 1, 8, 16, 4)])
+def test_more_threads_than_a_launch_has_are_refused(lib, sizes):
+    a = _args()
+    a.B, a.Lq, a.Hq, a.Hkv, a.D, a.P, a.S = sizes
+    assert lib.hpmn_prefix_attn(C.byref(a), None) == -2
+
+
 def test_struct_layout(tmp_path):
     st = _lib.HpmnPrefixAttn
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "hpmn_hip.h"', 'int main(void){printf("%zu", sizeof(HpmnPrefixAttn));']
