@@ -17,14 +17,27 @@ AttnPlan attn_plan(const HpmnPrefixAttn &a) {
     p.d4 = (a.D + 3) / 4 * 4;
     p.mw_pre = M > 64 ? 4 : 2;
     p.mw_suf = per_seq > 64 ? 4 : 2;
-    auto split = [&](long base, int keys, int tile, int &splits, int &per) {
+    p.rt_suf = a.S > 0 ? (int)((per_seq + 32 * p.mw_suf - 1) / (32 * p.mw_suf)) : 0;
+    // Few keys of very many sequences: the second kernel's, which asks for them beside the parts.  A workgroup for each costs its
+    // start and its own part: 300 x 8 heads of 128 over 4096 keys + 1 45.6 -> 27.6 us, 1000 x 16 heads over 2 of 128, 2048 + 8
+    // 75.0 -> 62.8, 64 x 8 heads of 128, 4096 + 1 22.6 -> 18.8; up to 512 of them run beside the prefix's (500 x 1 head of 64,
+    // 1000 + 1 11.3 against 11.7, 8 x 8 heads over 1 of 64 12.1 against 12.7).
+    long own = (long)a.B * a.Hkv * p.rt_suf;             // (sequence, key head, row tile)s with own keys
+    if (a.S <= JOIN_KEYS && own >= 512) {
+        p.keys = a.S;
+        own = 0;
+    }
+    auto split = [&](long base, int keys, int tile, long beside, int &splits, int &per) {
         const int tiles = std::max(1, (keys + tile - 1) / tile);
         // Keys: one workgroup per CU, two when each still has 1280 keys (fp32: 320) to work through -- a tile's loads hide behind the
         // other's products, shorter ranges pay more for their start and for the join: 300 x 8 heads of 128, 16384 keys 54 -> 50 us with
         // two, 200 x 8 heads over 2 of 64, 4096 keys 17.5 -> 21.  At most 128 parts to join (fp32, whose ranges cost more: 256):
         // 8 x 8 heads over 1 of 64, 32768 keys 13.8 us against 15.3 with 256 and 15.8 with 64; fp32, 8 rows 20.9 against 16.5 with 256.
         splits = (int)std::max<long>(1, std::min<long>(tiles, 256 / base));
-        if ((long)tiles * tile / splits >= (esize == 4 ? 320 : 1280)) splits = (int)std::max<long>(1, std::min<long>(tiles, 512 / base));
+        // Many workgroups of own keys hide beside one of the prefix on a CU: two of the prefix only for so much longer ranges (512 x 16
+        // heads over 4 of 128, + 64 own keys: 8192 keys 76.6 us with two, 65.1 with one; 32768 keys 172 against 189).
+        if ((long)tiles * tile / splits * 512 >= (esize == 4 ? 320 : 1280) * std::max(512l, beside))
+            splits = (int)std::max<long>(1, std::min<long>(tiles, 512 / base));
         splits = std::min(splits, esize == 4 ? 256 : 128);
         per = (tiles + splits - 1) / splits * tile;
         splits = std::max(1, (keys + per - 1) / per);
@@ -35,25 +48,16 @@ AttnPlan attn_plan(const HpmnPrefixAttn &a) {
     const bool whole = a.S == 0 && esize == 2 && (long)a.P * a.D <= (p.mw_pre == 4 ? 256 : 512) * 64;
     p.rt_pre = (int)((M + 32 * p.mw_pre - 1) / (32 * p.mw_pre));
     // (16-bit, many rows: pairs of tiles)
-    split((long)p.rt_pre * a.Hkv, a.P, attn_tile(esize, p.mw_pre) * (esize == 2 && p.mw_pre == 4 ? 2 : 1), p.splits_pre, p.per_pre);
+    split((long)p.rt_pre * a.Hkv, a.P, attn_tile(esize, p.mw_pre) * (esize == 2 && p.mw_pre == 4 ? 2 : 1), own, p.splits_pre,
+          p.per_pre);
     if (whole) {
         p.splits_pre = 1;
         p.per_pre = std::max(a.P, 1);
     }
     p.blocks_pre = (unsigned)(((long)a.Hkv * p.splits_pre + 7) / 8 * 8 * p.rt_pre);
-    if (a.S > 0) {
-        p.rt_suf = (int)((per_seq + 32 * p.mw_suf - 1) / (32 * p.mw_suf));
-        const long base = (long)a.B * a.Hkv * p.rt_suf;
-        // Few keys of very many sequences: the second kernel's, which asks for them beside the parts.  A workgroup for each costs its
-        // start and its own part: 300 x 8 heads of 128 over 4096 keys + 1 45.6 -> 27.6 us, 1000 x 16 heads over 2 of 128, 2048 + 8
-        // 75.0 -> 62.8, 64 x 8 heads of 128, 4096 + 1 22.6 -> 18.8; up to 512 of them run beside the prefix's (500 x 1 head of 64,
-        // 1000 + 1 11.3 against 11.7, 8 x 8 heads over 1 of 64 12.1 against 12.7).
-        if (a.S <= JOIN_KEYS && base >= 512) {
-            p.keys = a.S;
-        } else {
-            split(base, a.S, attn_tile(esize, p.mw_suf), p.splits_suf, p.per_suf);
-            p.blocks_suf = (unsigned)(base * p.splits_suf);
-        }
+    if (own > 0) {
+        split(own, a.S, attn_tile(esize, p.mw_suf), 0, p.splits_suf, p.per_suf);
+        p.blocks_suf = (unsigned)(own * p.splits_suf);
     }
     p.parts = p.splits_pre + p.splits_suf;
     p.join = p.parts > 1 || p.keys > 0;
