@@ -7,7 +7,9 @@
 //   the runs of a wave are scanned with lane shuffles, the waves of a tile through LDS (one barrier per tile, two buffers);
 //   the carried state enters, the run is replayed from it and stored.
 // z and v are read once, y is written once, nothing else reaches memory (training: one fp32 row per tile and channel).  Bound
-// by memory: the next tile's rows are in flight while this one is composed.
+// by memory: the next tile's rows are in flight while this one is composed.  Tiles of 128 steps because that is what one barrier
+// pays for at 512 threads (8 waves x 4 runs of 4); runs of 4 because z, v and the two gates of a run then fit 64 registers, two
+// workgroups a CU.
 // The backward walks the tiles in reverse.  Its scan G -> a (G + d_y) has the SAME a as the forward's, so one exchange serves
 // both: the states are recomputed from the tile's saved first row instead of being stored (a read of z and v, which d_z and d_v
 // need anyway, against a write and a read of all states in fp32).
@@ -132,6 +134,8 @@ struct ChunkArgs {
     int chunks, tiles;                       // per sequence, per chunk
 };
 
+// Bound by memory latency more than rate (a lane group walks its span alone, loads four steps ahead): 1 x 65536 x 256 bf16 14.8 us
+// for 67 MB, 4.5 TB/s; behind it the main kernel finds z and v in the cache, 24.2 us.
 template <typename T, int LPR, bool VEC, bool BWD>
 __global__ __launch_bounds__(512) void gated_scan_chunk_kernel(const ChunkArgs a) {
     constexpr int TG = 64 / LPR;
@@ -252,6 +256,8 @@ __device__ __forceinline__ v4f fold_chunks(const float *ws, int C, int c, int nl
     return start;
 }
 
+// Memory-bound: 500 x 1024 x 64 fp32, period 2, 328 MB in 71.6 us, 4.6 TB/s (a copy reaches 4.7); 16 x 4096 x 1024 bf16, 403 MB in
+// 81.4 us, 4.9 TB/s.  Small calls are a launch and one round trip to memory: 128 x 100 x 32 fp32 4.9 us.
 template <typename T, int LPR, bool VEC>
 __global__ __launch_bounds__(512) void gated_scan_fwd_kernel(const HpmnGatedScan a, int chunks, int chunk_tiles) {
     constexpr int TG = 64 / LPR;             // runs side by side in a wave
@@ -331,6 +337,8 @@ __global__ __launch_bounds__(512) void gated_scan_fwd_kernel(const HpmnGatedScan
     if (a.h_last && chunk == chunks - 1 && threadIdx.x < LPR) store_state(a.h_last + b * a.C + sh.c, carry, sh.n);
 }
 
+// Memory-bound: 500 x 1024 x 64 fp32, period 2, 590 MB in 105.9 us, 5.6 TB/s; 16 x 4096 x 1024 bf16, 671 MB in 149 us, 4.5 TB/s
+// (256 workgroups there, one a CU, whose waves wait for memory half of their cycles); 128 x 100 x 32 fp32 6.6 us.
 template <typename T, int LPR, bool VEC>
 __global__ __launch_bounds__(512) void gated_scan_bwd_kernel(const HpmnGatedScanBwd a, int chunks, int chunk_tiles) {
     constexpr int TG = 64 / LPR;
@@ -457,36 +465,67 @@ __device__ __forceinline__ long step_user(const HpmnGatedStep &a, int b) {
     return (a.flags & HPMN_STEP_USER_I64) ? (long)((const int64_t *)a.user)[b] : (long)((const int32_t *)a.user)[b];
 }
 
-// One wave per row.  With HPMN_STEP_COMMIT and a user list, the FIRST row that names a user carries out all rows of that user,
-// in row order; the others find an earlier row with their user and leave.
+// Row j's event on user u's state by one wave; a lane's channels are its own, so the next event of the user sees what this one left.
+// Scalar accesses: two dependent round trips (index, then state) are the time, whatever their width.
+template <typename T>
+__device__ __forceinline__ void step_event(const HpmnGatedStep &a, int lane, int j, long u) {
+    for (int c = lane; c < a.C; c += 64) {
+        float ag, ug;
+        gate_pair((float)((const T *)a.z)[j * a.z_s + c], ag, ug);
+        const float h = fmaf(ag, a.state[u * a.state_s + c], ug * (float)((const T *)a.v)[j * a.v_s + c]);
+        if (a.y) ((T *)a.y)[j * a.y_s + c] = (T)h;
+        if (a.flags & HPMN_STEP_COMMIT) a.state[u * a.state_s + c] = h;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void step_unknown(const HpmnGatedStep &a, int lane, int j) {
+    if (a.y)
+        for (int c = lane; c < a.C; c += 64) ((T *)a.y)[j * a.y_s + c] = (T)__builtin_nanf("");
+}
+
+// Rows that do not wait for each other: a wave each.  Bound by its launch and the round trips: one row of 64 fp32 1.4 us, 4096 rows of
+// 128 bf16 3.8 us of device time, against the 8 us that the host takes for the call.
 template <typename T>
 __global__ __launch_bounds__(64) void gated_step_kernel(const HpmnGatedStep a) {
     const int b = blockIdx.x, lane = threadIdx.x;
     const long u = step_user(a, b);
-    const bool ordered = (a.flags & HPMN_STEP_COMMIT) && a.user;
-    if (u < 0 || u >= a.n_users) {
-        if (a.y)
-            for (int c = lane; c < a.C; c += 64) ((T *)a.y)[b * a.y_s + c] = (T)__builtin_nanf("");
-        return;
-    }
-    if (ordered) {
-        bool earlier = false;
-        for (int j = lane; j < b; j += 64) earlier |= step_user(a, j) == u;
-        if (__any(earlier)) return;
-    }
-    for (int c0 = 0; c0 < a.C; c0 += 64) {
-        const int c = c0 + lane;
-        const bool on = c < a.C;
-        float h = on ? a.state[u * a.state_s + c] : 0.f;
-        for (int j = b; j < (ordered ? a.B : b + 1); ++j) {
-            if (j > b && step_user(a, j) != u) continue;
-            if (!on) continue;
-            float ag, ug;
-            gate_pair((float)((const T *)a.z)[j * a.z_s + c], ag, ug);
-            h = fmaf(ag, h, ug * (float)((const T *)a.v)[j * a.v_s + c]);
-            if (a.y) ((T *)a.y)[j * a.y_s + c] = (T)h;
+    if (u < 0 || u >= a.n_users) step_unknown<T>(a, lane, b);
+    else step_event<T>(a, lane, b, u);
+}
+
+// HPMN_STEP_COMMIT with a user list: the FIRST row that names a user carries out all rows of that user, in row order; the others find
+// an earlier row with their user and leave.  A wave per row; eight of them read the list together, a part at a time through LDS, and
+// compare 512 users before they look at the outcome, which is nothing most of the time.  4096 rows of 128 bf16 8.8 us (a branch
+// for every 64 users: 22.5; every wave reading by itself: 18.5; a row at a time: 880).
+template <typename T, typename U>
+__global__ __launch_bounds__(512) void gated_step_ordered_kernel(const HpmnGatedStep a) {
+    constexpr int PART = 2048, LOOK = 8;
+    __shared__ U named[PART];
+    const int lane = threadIdx.x & 63, b = blockIdx.x * 8 + (threadIdx.x >> 6);
+    const U *users = (const U *)a.user, u = users[min(b, a.B - 1)];
+    bool done = b >= a.B || u < 0 || (long)u >= a.n_users;
+    if (b < a.B && done) step_unknown<T>(a, lane, b);
+    for (int j0 = 0; j0 < a.B; j0 += PART) {
+        if (j0 > 0) __syncthreads();
+        for (int i = threadIdx.x; i < PART; i += 512) named[i] = j0 + i < a.B ? users[j0 + i] : (U)-1;      // (-1: no row's user)
+        __syncthreads();
+        if (done) continue;
+        for (int i = 0; i < min(PART, a.B - j0) && !done; i += 64 * LOOK) {
+            uint64_t same[LOOK], any = 0;
+#pragma unroll
+            for (int k = 0; k < LOOK; ++k) {
+                same[k] = __ballot(named[i + 64 * k + lane] == u);
+                any |= same[k];
+            }
+            if (any == 0) continue;
+#pragma unroll
+            for (int k = 0; k < LOOK; ++k) {
+                const int before = b - (j0 + i + 64 * k);    // rows of these in front of this wave's
+                if (before > 0 && (before >= 64 ? same[k] : same[k] & ((1ull << before) - 1))) done = true;
+                if (!done)
+                    for (uint64_t s = same[k]; s; s &= s - 1) step_event<T>(a, lane, j0 + i + 64 * k + __builtin_ctzll(s), (long)u);
+            }
         }
-        if (on && (a.flags & HPMN_STEP_COMMIT)) a.state[u * a.state_s + c] = h;
     }
 }
 
@@ -590,11 +629,19 @@ int gated_scan_bwd_launch(const HpmnGatedScanBwd &a, hipStream_t st) {
     return check_launch();
 }
 
+template <typename T>
+static void step_type(const HpmnGatedStep &a, hipStream_t st) {
+    const dim3 eighths((unsigned)((a.B + 7) / 8));
+    const bool ordered = (a.flags & HPMN_STEP_COMMIT) && a.user;
+    if (ordered && (a.flags & HPMN_STEP_USER_I64)) hipLaunchKernelGGL((gated_step_ordered_kernel<T, int64_t>), eighths, dim3(512), 0, st, a);
+    else if (ordered) hipLaunchKernelGGL((gated_step_ordered_kernel<T, int32_t>), eighths, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL(gated_step_kernel<T>, dim3((unsigned)a.B), dim3(64), 0, st, a);
+}
+
 int gated_step_launch(const HpmnGatedStep &a, hipStream_t st) {
-    const dim3 grid((unsigned)a.B);
-    if (a.dtype == HPMN_F32) hipLaunchKernelGGL(gated_step_kernel<float>, grid, dim3(64), 0, st, a);
-    else if (a.dtype == HPMN_BF16) hipLaunchKernelGGL(gated_step_kernel<bf16_t>, grid, dim3(64), 0, st, a);
-    else hipLaunchKernelGGL(gated_step_kernel<f16_t>, grid, dim3(64), 0, st, a);
+    if (a.dtype == HPMN_F32) step_type<float>(a, st);
+    else if (a.dtype == HPMN_BF16) step_type<bf16_t>(a, st);
+    else step_type<f16_t>(a, st);
     return check_launch();
 }
 

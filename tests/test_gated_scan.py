@@ -428,6 +428,34 @@ def test_step_orders_events_of_one_user(width):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("width", [torch.int32, torch.int64])
+@pytest.mark.parametrize("B", [1, 7, 9, 64, 511, 513, 2047, 2049, 4096])
+def test_step_commits_distinct_users_and_a_late_repeat(width, B):
+    """Every user once, then the first row's user again in the last row; an unknown user in between (int64: one whose low half
+    is a known user's): equal to the uncommitted step of each row, bit for bit."""
+    Cc, U = 70, 5000
+    z, v = (t[:, 0] for t in inputs(B, 1, Cc, torch.bfloat16))
+    user = torch.randperm(U, generator=torch.Generator().manual_seed(B))[:B].to("cuda", width)
+    state = torch.randn(U, Cc, generator=torch.Generator().manual_seed(2)).cuda()
+    if B > 8:
+        user[-1] = user[0]
+        user[5] = -1 if width == torch.int32 else (1 << 32) + int(user[6])
+    want, alone = state.clone(), ops.gated_scan_step(z, v, state, user, commit=False)
+    y = ops.gated_scan_step(z, v, state, user)
+    known = [b for b in range(B) if 0 <= int(user[b]) < U]
+    n = len(known) - (1 if B > 8 else 0)
+    assert torch.equal(y[known[:n]], alone[known[:n]])
+    if B > 8:
+        assert torch.isnan(y[5]).all()
+        first = ops.gated_scan_step(z[:1].float(), v[:1].float(), want[user[0]][None], commit=False)
+        last = ops.gated_scan_step(z[-1:].float(), v[-1:].float(), first, commit=False)
+        assert torch.equal(state[user[0]], last[0]) and torch.equal(y[-1], last[0].bfloat16())
+    untouched = torch.ones(U, dtype=torch.bool, device="cuda")
+    untouched[user[known].long()] = False
+    assert torch.equal(state[untouched], want[untouched])
+
+
+@pytest.mark.gpu
 def test_step_reads_only_without_commit_and_skips_unknown_users():
     z, v = (t[:, 0] for t in inputs(6, 1, 16, torch.float32))
     state = torch.randn(3, 16, device="cuda")
