@@ -111,3 +111,44 @@ def test_candidates_are_ranked_against_one_history(T, N):
     assert torch.equal(y1, own[:1]) and not torch.equal(store, before)
     z2, v2 = torch.cat([z, zc[None, :1]], 1), torch.cat([v, vc[None, :1]], 1)
     assert (ops.gated_scan_fwd(z2, v2)[1] - store).abs().max() < 1e-5
+
+
+@pytest.mark.gpu
+def test_calls_side_by_side_and_two_graphs_do_not_meet():
+    """The same operators on two streams at once, and in two captured graphs replayed in turn with eager calls between: every
+    call has workspace of its own."""
+    g = torch.Generator().manual_seed(4)
+    f = lambda *s: torch.randn(*s, generator=g).cuda().bfloat16()  # noqa: E731
+    sets = []
+    for B, P, T in ((40, 5000, 2000), (90, 3300, 1500)):
+        sets.append((f(B, 1, 4, 64), f(P, 2, 64), f(P, 2, 64), f(B, 20, 2, 64), f(B, 20, 2, 64), f(3, T, 64), f(3, T, 64)))
+
+    def run(x):
+        q, kp, vp, ks, vs, z, v = x
+        return ops.shared_prefix_attention(q, kp, vp, ks, vs), *ops.gated_scan_fwd(z, v)[:2]
+
+    want = [run(x) for x in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(4):
+        for i, x in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(x))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for r in got[i] for a, b in zip(r, want[i]))
+    graphs, held = [], []
+    for x in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(run(x))
+    for k in range(3):
+        for i in (0, 1, 0):
+            for h in held[i]:
+                h.zero_()
+            graphs[i].replay()
+            eager = run(sets[1 - i])
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(held[i], want[i])), (k, i)
+            assert all(torch.equal(a, b) for a, b in zip(eager, want[1 - i])), (k, i)
