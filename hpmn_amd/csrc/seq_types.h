@@ -15,13 +15,17 @@ template <> struct Quad<float> { typedef v4f type; };
 template <> struct Quad<bf16_t> { typedef bf16x4 type; };
 template <> struct Quad<f16_t> { typedef f16x4 type; };
 template <typename T> using quad_t = typename Quad<T>::type;
+// the same in memory, aligned to an element: one access all the same (global memory takes any alignment; across cache lines it costs
+// a second one)
+template <typename T> struct LooseQuad { typedef quad_t<T> type __attribute__((aligned(sizeof(T)))); };
+template <typename T> using loose_quad_t = typename LooseQuad<T>::type;
 
-// Four elements from p on (VEC: one aligned access), or the n in 1..4 valid ones of them (!VEC: scalar accesses; the rest repeat
-// the last valid one).  Unconditional in every lane: a load under a condition is waited for where the paths meet.
+// Four elements from p on (VEC: one access), or the n in 1..4 valid ones of them (!VEC: scalar accesses; the rest repeat the last
+// valid one).  Unconditional in every lane: a load under a condition is waited for where the paths meet.
 template <typename T, bool VEC>
 __device__ __forceinline__ quad_t<T> load_quad(const T *p, int n) {
     if constexpr (VEC) {
-        return *reinterpret_cast<const quad_t<T> *>(p);
+        return *reinterpret_cast<const loose_quad_t<T> *>(p);
     } else {
         quad_t<T> q;
 #pragma unroll
@@ -32,7 +36,7 @@ __device__ __forceinline__ quad_t<T> load_quad(const T *p, int n) {
 template <typename T, bool VEC>
 __device__ __forceinline__ void store_quad(T *p, v4f x, int n) {
     if constexpr (VEC) {
-        *reinterpret_cast<quad_t<T> *>(p) = __builtin_convertvector(x, quad_t<T>);
+        *reinterpret_cast<loose_quad_t<T> *>(p) = __builtin_convertvector(x, quad_t<T>);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
