@@ -548,11 +548,14 @@ struct Cut {
 //   8 x 1024: 11 / 14 against 19 / 28;   64 x 4096: 55 / 80 against 65 / 130;   1 x 16384: 14 / 17 against 241 / 379;
 //   at the rule's borders: 64 x 512 12.4 / 17.1 against 11.7 / 17.6, 80 x 1024 19 / 27 against 20 / 31;
 //   beyond them: 96 x 1024 (two chunks) 26 / 33 against 21 / 32, 8 x 256 (two tiles) 10 / 12 against 7 / 10.
+// Up to 32 (16) channels a workgroup has half (a quarter) of the waves, so the CUs are full with twice (four times) as many:
+//   49 x 7701 x 10 bf16 20 / 28 against 35 / 48 with 256, 64 x 4096 x 16 fp32 20 / 27 against 27 / 32, 84 x 1024 x 32 15.4 / 20.9 against
+//   15.2 / 20.0.
 static Cut scan_cut(int B, int T, int C) {
     const int lpr = scan_lanes(C), tiles = (T + TILE - 1) / TILE;
     const long whole = (long)B * ((C + 4 * lpr - 1) / (4 * lpr));
-    const int want = (int)std::min<long>(std::min(tiles, TILE), 256 / whole);
-    if (want < 3 || tiles < 4) return {1, tiles};
+    if (256 / whole < 3 || tiles < 4) return {1, tiles};
+    const int want = (int)std::min<long>(std::min(tiles, TILE), 256 * 16 / lpr / whole);
     const int per = (tiles + want - 1) / want;
     return {(tiles + per - 1) / per, per};
 }
