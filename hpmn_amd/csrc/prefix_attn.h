@@ -12,7 +12,8 @@
 // permuted by the row number so that neither the reads along a row nor those across sixteen rows meet in a bank.
 // Few rows: the waves of a workgroup share out the keys of a tile two by two and join their results in LDS.  The key
 // axis is split over workgroups until the chip is full; a second kernel joins the parts (maximum, sum, unnormalised output in fp32).
-// A row's own suffix is the same thing with M = Lq Hq / Hkv rows and a key limit per row, in the same launch.
+// A row's own suffix is the same thing with M = Lq Hq / Hkv rows and a key limit per row, in the same launch; a few keys of very many
+// sequences are left to the joining kernel.
 //
 // Bound by the matrix pipe for many rows: 512 x 16 heads over 4 of 128, 32768 keys + 64 own bf16, 137.6 GF: 160 us + 9.7 us of joining,
 // 0.86 PF/s in the first kernel (a library product of 8192^3 1.22; what is missing: the probabilities' share of issue slots, and the
