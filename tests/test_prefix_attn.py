@@ -375,3 +375,107 @@ def test_prefix_and_suffix_agree():
         ks, vs = (t[None, cut:].expand(5, 96 - cut, 2, 64) for t in (kp, vp))
         got = check(q, kp[:cut], vp[:cut], ks, vs)
         assert (got[0] - want[0]).abs().max() < 2e-6 and (got[1] - want[1]).abs().max() < 2e-6
+
+
+# ------------------------------------------------------------------------------ many rows: the pipelined whole tiles
+def many_rows_check(q, kp, vp, scale, plen=None):
+    """q [M, 1, H, D] over H key heads of their own against float64 on the GPU; the tolerances of check()."""
+    dt, (M, _, H, D) = q.dtype, q.shape
+    p = kp.shape[0] if plen is None else plen
+    out, lse = ops.shared_prefix_attention(q, kp, vp, prefix_len=None if plen is None else i32(plen), scale=scale, want_lse=True)
+    assert torch.equal(ops.shared_prefix_attention(q, kp, vp, prefix_len=None if plen is None else i32(plen), scale=scale), out)
+    half = torch.finfo(dt).eps / 2
+    for h0 in range(0, H, 32):
+        part = slice(h0, min(H, h0 + 32))
+        k = kp[:p, part].double().permute(1, 2, 0).contiguous()
+        v = vp[:p, part].double().permute(1, 0, 2).contiguous()
+        s = scale * torch.bmm(q[:, 0, part].double().transpose(0, 1).contiguous(), k)
+        wlse = torch.logsumexp(s, -1)
+        w = torch.exp(s - wlse[..., None])
+        want, spread = torch.bmm(w, v), torch.bmm(w, v.abs())
+        got = out[:, 0, part].double().transpose(0, 1)
+        over = (got - want).abs() - (half * (want.abs() + spread) + 6e-5 * spread + 1e-7)
+        assert over.max() <= 0, "heads from %d: off by %.3g, %.3g over" % (h0, (got - want).abs().max(), over.max())
+        l = lse[:, 0, part].double().transpose(0, 1)
+        assert ((l - wlse).abs() <= 6e-5 + 2e-7 * wlse.abs()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [32, 40, 64, 72, 96, 128])
+@pytest.mark.parametrize("P", [356, 421, 640, 1100, 2200])
+def test_long_ranges_of_many_rows(P, D, dtype):
+    """256 key heads fill the chip, so a range of keys is long: four, six, ten, sixteen and eighteen tiles of 64 in one go, with and
+    without a rest; and the same with the prefix cut at the device."""
+    dt = DTYPES[dtype]
+    g = torch.Generator(device="cuda").manual_seed(P + D)
+    M = 66 if D >= 96 else 128
+    q = (1.5 * torch.randn(M, 1, 256, D, device="cuda", generator=g)).to(dt)
+    kp, vp = (torch.randn(P, 256, D, device="cuda", generator=g).to(dt) for _ in range(2))
+    many_rows_check(q, kp, vp, D ** -0.5)
+    many_rows_check(q, kp, vp, -D ** -0.5, plen=P - 70)
+    kp[P - 70:] = float("nan")
+    vp[P - 70:] = float("inf")
+    want = ops.shared_prefix_attention(q, kp[:P - 70], vp[:P - 70])
+    got = ops.shared_prefix_attention(q, kp, vp, prefix_len=i32(P - 70))
+    assert (got.double() - want.double()).abs().max() <= 4 * torch.finfo(dt).eps * float(want.double().abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_rising_maxima_of_many_rows(D, dtype):
+    """The running maximum rises by 1 to 120 (in powers of two) at every step of 32 keys of a range in turn -- the first and
+    the second of a tile, across pairs of tiles, in the last one -- once, or at every step, so that it lags, is raised and rescales
+    the output late.  Rows see the keys as they rise, as they fall, half as far apart and all alike."""
+    dt, P, H, M = DTYPES[dtype], 1100, 256, 72
+    g = torch.Generator(device="cuda").manual_seed(D)
+    rises = torch.tensor([1.0, 2.5, 4.0, 7.0, 9.0, 20.0, 120.0], device="cuda")
+    step = torch.arange(P, device="cuda") // 32                        # 0 .. 34
+    level = torch.zeros(P, H, device="cuda")
+    for h in range(H):
+        r, at = rises[h % 7], h // 7 % 35
+        level[:, h] = (step >= at) * r if h < 245 else step * r
+    q = torch.zeros(M, 1, H, D, device="cuda", dtype=dt)
+    q[:, :, :, 0] = torch.tensor([1.0, -1.0, 0.5, 0.0], device="cuda", dtype=dt).repeat(M // 4)[:, None, None]
+    q[0::5, :, :, 0] = 1.0
+    kp = torch.zeros(P, H, D, device="cuda", dtype=dt)
+    kp[:, :, 0] = (level + 0.5 * torch.randn(P, H, device="cuda", generator=g)).to(dt)
+    vp = torch.randn(P, H, D, device="cuda", generator=g).to(dt)
+    many_rows_check(q, kp, vp, math.log(2.0))
+
+
+@pytest.mark.parametrize("sizes,splits", [((8, 1, 1, 1, 64, 1000, 0), True), ((1, 1, 1, 1, 128, 1 << 20, 0), True), ((3, 9, 8, 2, 40, 5000, 77), True),
+                                          ((500, 1, 16, 4, 128, 32768, 64), True), ((300, 1, 8, 8, 128, 4096, 1), True),
+                                          ((2, 1, 4, 2, 64, 100, 0), False), ((1, 1, 1, 1, 32, 0, 0), False)])
+def test_long_prefixes_and_own_keys_are_cut_up(lib, sizes, splits):
+    """Where keys are to be shared out a workspace is asked for, and has to be there, large enough and aligned; a short prefix by
+    itself needs none."""
+    a = _args()
+    a.B, a.Lq, a.Hq, a.Hkv, a.D, a.P, a.S = sizes
+    need = lib.hpmn_prefix_attn_workspace_bytes(C.byref(a))
+    assert (need > 0) == splits
+    for ws, n in ((None, need), (4096, need - 1), (4104, need)) if splits else ():
+        a.workspace, a.workspace_bytes = ws, n
+        assert lib.hpmn_prefix_attn(C.byref(a), None) == -1
+
+
+@pytest.mark.gpu
+def test_refusals_are_value_errors():
+    """Every bad argument is refused by name, none by an accident further in."""
+    z = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+    q, kp, ks = z(2, 1, 4, 64), z(9, 2, 64), z(2, 5, 2, 64)
+    n = lambda *s, dtype=torch.int32: torch.zeros(*s, device="cuda", dtype=dtype)  # noqa: E731
+    f = ops.shared_prefix_attention
+    for i, call in enumerate([lambda: f(q[0], kp, kp), lambda: f(q, kp, kp[:8]), lambda: f(q, kp.half(), kp.half()),
+                              lambda: f(q.double(), kp.double(), kp.double()), lambda: f(q, kp.cpu(), kp), lambda: f(q, kp, kp, ks),
+                              lambda: f(q, kp, kp, None, ks), lambda: f(q, kp, kp, ks[:1], ks[:1]), lambda: f(q, kp, kp, ks, ks[:, :4]),
+                              lambda: f(q, kp, kp, ks[0], ks[0]), lambda: f(q[:, :, :3], kp, kp), lambda: f(q[..., :32], kp, kp),
+                              lambda: f(q, kp, kp, scale=float("nan")), lambda: f(q, kp, kp, scale=float("inf")),
+                              lambda: f(q, kp, kp, prefix_len=n(1, dtype=torch.int64)), lambda: f(q, kp, kp, prefix_len=5),
+                              lambda: f(q, kp, kp, prefix_len=n(2)), lambda: f(q, kp, kp, ks, ks, suffix_len=n(3)),
+                              lambda: f(q, kp, kp, ks, ks, suffix_len=[1, 2]), lambda: f(z(2, 1, 4, 160), z(9, 2, 160), z(9, 2, 160)),
+                              lambda: f(q.transpose(2, 3), z(9, 2, 4), z(9, 2, 4)), lambda: f(q, kp[:, :0], kp[:, :0]), lambda: f(q, kp[0], kp[0])]):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail("call %d was accepted" % i)
