@@ -441,19 +441,27 @@ __global__ __launch_bounds__(512) void gated_scan_bwd_kernel(const HpmnGatedScan
         }
         if (tg > 0) h = Ae * h + Be;
         if (tg < TG - 1) G = Ax * G + Bx;
-        v4f hp[RUN];
 #pragma unroll
-        for (int s = 0; s < RUN; ++s) {
-            hp[s] = h;
-            h = ag[s] * h + ug[s] * vv[s];
+        for (int s = 0; s < RUN; ++s) {                      // h_{t-1} - v in v's place
+            const v4f x = vv[s];
+            vv[s] = h - x;
+            h = ag[s] * h + ug[s] * x;
         }
 #pragma unroll
         for (int s = RUN - 1; s >= 0; --s) {
             G += dd[s];
-            const v4f gv = ug[s] * G;
+            v4f gv = ug[s] * G;
+            if (!whole) {                                    // steps that do not count: zeros, also where G or h is no number
+                const bool live = sh.live(t + s);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    gv[i] = live ? gv[i] : 0.f;
+                    vv[s][i] = live ? vv[s][i] : 0.f;
+                }
+            }
             if (sh.n > 0 && t + s < sh.hi) {
                 store_quad<T, VEC>(at_row(dv, (unsigned)(t + s), a.dv_st), gv, sh.n);
-                store_quad<T, VEC>(at_row(dz, (unsigned)(t + s), a.dz_st), gv * ag[s] * (hp[s] - vv[s]), sh.n);
+                store_quad<T, VEC>(at_row(dz, (unsigned)(t + s), a.dz_st), gv * ag[s] * vv[s], sh.n);
             }
             G = ag[s] * G;
         }

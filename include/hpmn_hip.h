@@ -793,7 +793,7 @@ int hpmn_memory_update(const HpmnOnlineUpdate *args, void *stream);
  * z, v: [B, T, C] of `dtype`; element strides over b and t (below 2^31 over t) are arguments (two halves of one projection
  * buffer), the last dimension is dense.  States, gates and sums are fp32 whatever the dtype; y, d_z, d_v are rounded to it once.
  *   begin  : optional [B] int32: front padding.  Steps t < begin[b] are identities (h_t = h_{t-1}, whatever z and v hold
- *            there, NaN included) and have zero gradients; begin[b] >= T: nothing but padding.
+ *            there, NaN included) and have zero gradients (whatever d_y or the state is there); begin[b] >= T: nothing but padding.
  *   h0     : optional [B, C] (row stride h0_sb): the state in front of step 0; NULL: zero.
  *   y      : optional [B, T / period, C];  h_last: optional [B, C];  T % period == 0.
  *   saved  : optional [B, ceil(T / HPMN_GATED_SCAN_TILE), C]: the state in front of every tile of HPMN_GATED_SCAN_TILE

@@ -482,3 +482,27 @@ def test_events_fed_one_by_one_leave_the_scan_state():
         yt = ops.gated_scan_step(z[:, t], v[:, t], state)
         assert (yt - y[:, t]).abs().max() < 2e-6       # two orders of the same fp32 sums, |state| <= 1
     assert (state - h_last).abs().max() < 2e-6
+
+
+# ------------------------------------------------------------------------------------------------------ padding, long memory
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("B,T,Cc", [(4, 261, 48), (2, 1500, 37), (3, 40, 2)])
+def test_padded_steps_have_zero_gradients_whatever_arrives(B, T, Cc, dtype):
+    """d_z and d_v of the steps in front of `begin` are zeros also where d_y there, or the carried state, is infinite or NaN; the
+    steps behind do not notice."""
+    z, v = inputs(B, T, Cc, DTYPES[dtype])
+    begin = torch.tensor([T, T // 2, 0, 130][:B], dtype=torch.int32).clamp(max=T).cuda()
+    h0 = torch.randn(B, Cc, generator=torch.Generator().manual_seed(3)).cuda()
+    d_y = torch.randn(B, T, Cc, generator=torch.Generator().manual_seed(4)).to("cuda", DTYPES[dtype])
+    padded = torch.arange(T, device="cuda")[None] < begin[:, None]
+    _, _, saved = ops.gated_scan_fwd(z, v, h0=h0, begin=begin, train=True)
+    want = ops.gated_scan_bwd(z, v, saved, d_y, begin=begin)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        got = ops.gated_scan_bwd(z, v, saved, torch.where(padded[..., None], bad, d_y.float()).to(d_y.dtype), begin=begin)
+        for g, w in zip(got[:2], want[:2]):
+            assert not g[padded].any() and torch.equal(g, w), bad
+        _, h, s = ops.gated_scan_fwd(z, v, h0=torch.full_like(h0, bad), begin=begin, train=True)
+        assert not torch.isfinite(h[0]).any()                          # nothing but padding: the state as it came
+        got = ops.gated_scan_bwd(z, v, s, d_y, begin=begin)
+        assert not got[0][padded].any() and not got[1][padded].any(), bad
