@@ -8,8 +8,8 @@
 //   the carried state enters, the run is replayed from it and stored.
 // z and v are read once, y is written once, nothing else reaches memory (training: one fp32 row per tile and channel).  Bound
 // by memory: the next tile's rows are in flight while this one is composed.  Tiles of 128 steps because that is what one barrier
-// pays for at 512 threads (8 waves x 4 runs of 4); runs of 4 because z, v and the two gates of a run then fit 64 registers, two
-// workgroups a CU.
+// pays for at 512 threads (8 waves x 4 runs of 4); runs of 4 because the forward's rows, gates and maps of a run then fit 128
+// registers, two workgroups a CU; the backward has about 200 to 230 and one workgroup a CU.
 // The backward walks the tiles in reverse.  Its scan G -> a (G + d_y) has the SAME a as the forward's, so one exchange serves
 // both: the states are recomputed from the tile's saved first row instead of being stored (a read of z and v, which d_z and d_v
 // need anyway, against a write and a read of all states in fp32).
@@ -433,8 +433,12 @@ __global__ __launch_bounds__(512) void gated_scan_bwd_kernel(const HpmnGatedScan
         const v4f Ae = shfl_up4(Af, LPR), Be = shfl_up4(Bf, LPR);
         const v4f Ax = shfl_down4(Ar, LPR), Bx = shfl_down4(Br, LPR);
         lds_barrier();
+        // (four waves' maps in flight: unrolled further, as the compiler does by itself, they alone take 64 registers, and the
+        // fp32 form spills in this loop: 16 x 4096 x 1024 bf16 161 us against 150, 128 x 100 x 32 fp32 7.5 against 6.8)
         v4f h = h_tile, G = R;
+#pragma unroll 4
         for (int i = 0; i < w; ++i) h = buf[i][0][cg] * h + buf[i][1][cg];
+#pragma unroll 4
         for (int i = nw - 1; i >= 0; --i) {
             if (i == w) G = R;
             R = buf[i][0][cg] * R + buf[i][2][cg];

@@ -114,3 +114,36 @@ def test_read_training_launch_on_eight_waves_fits_the_register_file(tmp_path):
     for prefix in ("_ZN4hpmn19read_fwd_bwd_kernelILb0", "_ZN4hpmn15read_fwd_kernel"):
         regs, occ, scratch = facts(prefix)
         assert regs <= 256 and occ >= 2 and scratch == 0, (prefix, regs, occ, scratch)
+
+
+def _product_assembly(tmp_path, name):
+    """As the library compiles it: with the source's own flags."""
+    from hpmn_amd import build
+    if not os.path.exists(HIPCC):
+        pytest.skip("no hipcc")
+    src, out = os.path.join(ROOT, "hpmn_amd", "csrc", name + ".hip"), str(tmp_path / (name + ".s"))
+    subprocess.check_call([HIPCC] + build.BASE_FLAGS + ["-w", "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(ROOT, "hpmn_amd", "csrc"),
+                                                        "-S", "--cuda-device-only", "-o", out] + build.file_flags(src) + [src])
+    with open(out) as f:
+        return f.read()
+
+
+def test_gated_scans_keep_nothing_in_scratch(tmp_path):
+    """Every form of the recurrence's kernels: no scratch at all, the forward's two workgroups of eight waves on a CU (128
+    registers) and the backward's one (256)."""
+    import re
+
+    import check_resources
+    text = _product_assembly(tmp_path, "gated_scan")
+    assert "v_pk_fma_f32" not in text and "v_pk_mul_f32" not in text and "v_pk_add_f32" not in text
+    info = check_resources.kernel_info(text)
+    scratch = dict(re.findall(r"^\s+\.name:\s+(\S+)\s+\.private_segment_fixed_size:\s+(\d+)", text, re.M))
+    counted = {"gated_scan_fwd_kernel": 0, "gated_scan_bwd_kernel": 0, "gated_scan_chunk_kernel": 0}
+    for name, (total, occupancy, loops) in info.items():
+        for kind in counted:
+            if kind in name:
+                counted[kind] += 1
+                assert int(scratch[name]) == 0 and not loops, name
+                assert total <= (256 if "bwd" in kind else 128), "%s: %d registers" % (name, total)
+    # three types, three widths, whole quads or not; the chunk kernel forward and backward
+    assert counted == {"gated_scan_fwd_kernel": 18, "gated_scan_bwd_kernel": 18, "gated_scan_chunk_kernel": 36}

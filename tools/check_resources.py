@@ -17,6 +17,9 @@ import sys
 import tempfile
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, ROOT)
+from hpmn_amd import build  # noqa: E402
+
 CSRC = os.path.join(ROOT, "hpmn_amd", "csrc")
 PAT = re.compile(r"\.name:\s+(\S+).*?\.private_segment_fixed_size:\s+(\d+).*?\.sgpr_count:\s+(\d+).*?"
                  r"\.sgpr_spill_count:\s+(\d+).*?\.vgpr_count:\s+(\d+).*?\.vgpr_spill_count:\s+(\d+)", re.S)
@@ -58,7 +61,7 @@ def main():
             out = os.path.join(tmp, os.path.basename(src) + ".s")
             subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-w",
                                    "-I" + os.path.join(ROOT, "include"), "-I" + CSRC, "-S", "--cuda-device-only",
-                                   "-o", out, src])
+                                   "-o", out] + build.file_flags(src) + [src])
             text = open(out).read()
             nflat = len(re.findall(r"^\s+flat_(?:load|store|atomic)", text, flags=re.M))
             if nflat:
