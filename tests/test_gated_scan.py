@@ -506,3 +506,33 @@ def test_padded_steps_have_zero_gradients_whatever_arrives(B, T, Cc, dtype):
         assert not torch.isfinite(h[0]).any()                          # nothing but padding: the state as it came
         got = ops.gated_scan_bwd(z, v, s, d_y, begin=begin)
         assert not got[0][padded].any() and not got[1][padded].any(), bad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("z0", [6.0, 8.0, 10.0, 12.0])
+@pytest.mark.parametrize("B,Cc", [(90, 64), (2, 64), (3, 20), (3, 10), (130, 9)])
+def test_long_memory(B, Cc, z0):
+    """Gates held near 1: a state remembers e^z steps, and 1 - a is a few parts in 10^5, which a rounded to fp32 near 1 (2^-25) carries
+    only to a few digits.  The decay over a wave's 16 or more steps is known to one rounding (2^-25), and the state is rounded once
+    (2^-24) when it is taken over them; per 16 steps of memory that adds up to 1.5 2^-24 of the state, over min(T, e^z) steps.  All
+    else (gates, the sums of a wave, the replay of four steps) is the constant of close(), 2e-5."""
+    T = 8192
+    g = torch.Generator().manual_seed(int(z0))
+    z = (z0 + 0.25 * torch.rand(B, 1, Cc, generator=g)).expand(B, T, Cc).contiguous().cuda()
+    v = (0.5 + 0.5 * torch.rand(B, T, Cc, generator=g)).cuda()         # (one sign: what is lost shows in the mean)
+    h0 = torch.rand(B, Cc, generator=g).cuda()
+    d_y = (0.5 + 0.5 * torch.rand(B, T // 64, Cc, generator=g)).cuda()
+    d_h = torch.rand(B, Cc, generator=g).cuda()
+    y, h_last, saved = ops.gated_scan_fwd(z, v, h0=h0, period=64, train=True)
+    d_z, d_v, d_h0 = ops.gated_scan_bwd(z, v, saved, d_y, d_h_last=d_h, period=64)
+    want = oracle(z, v, h0, None, 64, d_y, d_h)
+    tol = 2e-5 + 1.5 * 2.0 ** -24 * min(T, np.exp(z0 + 0.25)) / 16
+    for name, got in (("y", y), ("h_last", h_last)):
+        off = np.abs(got.double().cpu().numpy() - want[name]).max()
+        assert off <= tol, "%s: off by %.3g, %.3g allowed" % (name, off, tol)          # (|h|, |v| <= 1)
+    u = 1 / (1 + np.exp(z.double().cpu().numpy()))
+    G = want["d_v"] / u
+    size = np.abs(G).max()
+    for name, got, per in (("d_v", d_v, u), ("d_z", d_z, 2 * u * (1 - u)), ("d_h0", d_h0, 1.0)):
+        off = (np.abs(got.double().cpu().numpy() - want[name]) / per).max() / size
+        assert off <= tol, "%s: off by %.3g, %.3g allowed" % (name, off, tol)
