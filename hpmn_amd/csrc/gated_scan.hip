@@ -514,7 +514,9 @@ __device__ __forceinline__ void step_event(const HpmnGatedStep &a, int lane, int
     for (int c = lane; c < a.C; c += 64) {
         float ag, ug;
         gate_pair((float)((const T *)a.z)[j * a.z_s + c], ag, ug);
-        const float h = fmaf(ag, a.state[u * a.state_s + c], ug * (float)((const T *)a.v)[j * a.v_s + c]);
+        const float old = a.state[u * a.state_s + c], v = (float)((const T *)a.v)[j * a.v_s + c], d = v - old;
+        // a state that moves little moves by u (v - h): a rounded near 1 would pull it the same way at every event
+        const float h = ug < 0.5f && fabsf(d) < INFINITY ? fmaf(ug, d, old) : fmaf(ag, old, ug * v);
         if (a.y) ((T *)a.y)[j * a.y_s + c] = (T)h;
         if (a.flags & HPMN_STEP_COMMIT) a.state[u * a.state_s + c] = h;
     }

@@ -536,3 +536,40 @@ def test_long_memory(B, Cc, z0):
     for name, got, per in (("d_v", d_v, u), ("d_z", d_z, 2 * u * (1 - u)), ("d_h0", d_h0, 1.0)):
         off = (np.abs(got.double().cpu().numpy() - want[name]) / per).max() / size
         assert off <= tol, "%s: off by %.3g, %.3g allowed" % (name, off, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("z0", [4.0, 8.0, 10.0])
+@pytest.mark.parametrize("commit_list", [False, True])
+def test_events_of_a_long_memory(z0, commit_list):
+    """20000 events into stored states whose gates are held near 1, with and without a user list.  Every event rounds the state once,
+    by up to 2^-25 (states in [1/2, 1)), independently: the increments u (v - h) are many such steps.  Over the 1 / (2 u) events whose
+    squares add up that is 2^-25 sqrt(1 / 3) sqrt(1 / (2 u)); eight times that for the largest of 256 states, and the gate's own 2e-6
+    (|z| 2^-24 and a few roundings, relative to u)."""
+    U, Cc, T = 4, 64, 20000
+    g = torch.Generator().manual_seed(int(z0))
+    z = (z0 + 0.25 * torch.rand(U, Cc, generator=g)).cuda()
+    v = (0.5 + 0.5 * torch.rand(T, U, Cc, generator=g)).cuda()
+    state = (0.5 + 0.5 * torch.rand(U, Cc, generator=g)).cuda()
+    h = state.double().cpu().numpy()
+    user = torch.tensor([2, 0, 3, 1], dtype=torch.int32).cuda()
+    zd, vd = z.double().cpu().numpy(), v.double().cpu().numpy()
+    order = np.argsort(user.cpu().numpy())                             # row of every user
+    a, u = 1 / (1 + np.exp(-zd)), 1 / (1 + np.exp(zd))
+    for t in range(T):
+        ops.gated_scan_step(z, v[t], state, user if commit_list else None)
+        h = a[order] * h + u[order] * vd[t][order] if commit_list else a * h + u * vd[t]
+    off = np.abs(state.double().cpu().numpy() - h).max()
+    tol = 8 * 2.0 ** -25 * np.sqrt(1 / 3) * np.sqrt(1 / (2 * u.min())) + 2e-6
+    assert off <= tol, "off by %.3g, %.3g allowed" % (off, tol)
+
+
+@pytest.mark.gpu
+def test_step_on_infinite_states():
+    """An infinite state stays what the formula makes of it: infinite while a counts, also where 1 - a is zero."""
+    z = torch.tensor([[3.0, float("inf"), 200.0, 0.5, -2.0]]).cuda()
+    v = torch.ones(1, 5, device="cuda")
+    for bad in (float("inf"), -float("inf")):
+        state = torch.full((1, 5), bad, device="cuda")
+        y = ops.gated_scan_step(z, v, state)
+        assert (y == bad).all() and (state == bad).all()
