@@ -207,6 +207,7 @@ class HpmnTileFwd(C.Structure):
                 ("bc", C.c_void_p), ("y", C.c_void_p), ("h_last", C.c_void_p), ("h_last_stride", C.c_int64)]
 
 
+HPMN_EINVAL = -1
 HPMN_F32, HPMN_BF16, HPMN_F16 = 0, 1, 2
 HPMN_GATED_SCAN_TILE = 128
 HPMN_STEP_COMMIT = 1

@@ -1617,14 +1617,17 @@ def _seq_input(name, t, ndim):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _call_on(device, name, fn, a):
-    """fn(&a, stream) on the device's current stream, with that device current (a launch needs both to agree)."""
+def _call_on(device, name, fn, a, overlap=None):
+    """fn(&a, stream) on the device's current stream, with that device current (a launch needs both to agree).  ``overlap``: what an
+    invalid argument can only mean here, the others having been checked."""
     if device.index == torch.cuda.current_device():
         rc = fn(C.byref(a), _raw_stream(device.index))
     else:
         with torch.cuda.device(device):
             rc = fn(C.byref(a), _raw_stream(device.index))
     if rc != 0:
+        if overlap is not None and rc == _lib.HPMN_EINVAL:
+            raise ValueError(overlap)
         _lib.check(rc, name)
 
 
@@ -1680,7 +1683,7 @@ def gated_scan_fwd(z, v, *, h0=None, begin=None, period=1, train=False):
 def gated_scan_bwd(z, v, saved, d_y, *, d_h_last=None, begin=None, period=1, out=None):
     """hpmn_gated_scan_bwd: gradients of ``gated_scan_fwd`` (same ``z``, ``v``, ``begin``, ``period``; ``saved`` from its training
     form).  ``d_y`` [B, T/period, C] in z's dtype or None, ``d_h_last`` [B, C] float32 or None.  ``out`` = (d_z, d_v): buffers to
-    write into, e.g. the halves of one projection's gradient (strided), apart from the inputs and each other.  Returns (d_z, d_v, d_h0 float32 [B, C])."""
+    write into, e.g. the halves of one projection's gradient (strided), apart from the inputs and each other (refused otherwise).  Returns (d_z, d_v, d_h0 float32 [B, C])."""
     B, T, Cc, code, dev = _gated_scan_shape(z, v, begin, period)
     tiles = -(-T // _lib.HPMN_GATED_SCAN_TILE)
     if saved is None:
@@ -1718,7 +1721,7 @@ def gated_scan_bwd(z, v, saved, d_y, *, d_h_last=None, begin=None, period=1, out
                               v.stride(0), v.stride(1), _ptr(begin), saved.data_ptr(), _ptr(d_y), dy_sb, dy_st, _ptr(d_h_last),
                               d_z.data_ptr(), d_v.data_ptr(), d_z.stride(0), d_z.stride(1), d_v.stride(0), d_v.stride(1),
                               d_h0.data_ptr(), _ptr(ws), n)
-    _call_on(dev, "hpmn_gated_scan_bwd", _lib.load().hpmn_gated_scan_bwd, a)
+    _call_on(dev, "hpmn_gated_scan_bwd", _lib.load().hpmn_gated_scan_bwd, a, "out: d_z and d_v overlap each other or an input")
     return d_z, d_v, d_h0
 
 
@@ -1750,16 +1753,16 @@ def gated_scan_step(z, v, state, user=None, *, commit=True):
     zs, vs = z.stride(0), v.stride(0)
     a = _lib.HpmnGatedStep(B, Cc, code, flags, z.data_ptr(), v.data_ptr(), zs, vs, state.data_ptr(), max(state_s, Cc), users, _ptr(user),
                            y.data_ptr(), Cc)
-    fn = _lib.load().hpmn_gated_scan_step
+    fn, overlap = _lib.load().hpmn_gated_scan_step, "state: its memory is also z's, v's or user's"
     # the ordered form works through its user list in calls of HPMN_STEP_MAX_INDEXED rows (one stream: still in row order)
     most = _lib.HPMN_STEP_MAX_INDEXED
     if not (commit and user is not None and B > most):
-        _call_on(dev, "hpmn_gated_scan_step", fn, a)
+        _call_on(dev, "hpmn_gated_scan_step", fn, a, overlap)
         return y
     size, wide = z.element_size(), user.element_size()
     for lo in range(0, B, most):
         a.B = min(most, B - lo)
-        _call_on(dev, "hpmn_gated_scan_step", fn, a)
+        _call_on(dev, "hpmn_gated_scan_step", fn, a, overlap)
         a.z, a.v, a.y, a.user = a.z + most * zs * size, a.v + most * vs * size, a.y + most * Cc * size, a.user + most * wide
     return y
 

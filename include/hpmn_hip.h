@@ -801,7 +801,8 @@ int hpmn_memory_update(const HpmnOnlineUpdate *args, void *stream);
  * Backward, with G_t = dL/dh_t in full:
  *   G_t = d_y[fires at t] + a_{t+1} G_{t+1}  (+ d_h_last at T-1);   d_v = (1-a) G;   d_z = G (h_{t-1} - v) a (1-a);
  *   d_h0 = a_0 G_0.   Deterministic.  d_z / d_v / d_h0 are overwritten; d_y, d_h_last, d_h0 may be NULL (zero / not wanted).
- * No output overlaps an input or another output.  Calls of more work than one launch has threads for (2^32; at 512 threads per 64
+ * No output overlaps an input or another output (HPMN_EINVAL; columns of common rows, as in one projection's gradient, and parts of
+ * one buffer with the same strides are fine).  Calls of more work than one launch has threads for (2^32; at 512 threads per 64
  * channels of a sequence of 128 steps or more) are refused with HPMN_EUNSUPPORTED, here and in the calls below.
  * workspace: >= hpmn_gated_scan_workspace_bytes(B, T, C) bytes (16-byte aligned; may be 0 bytes: NULL then), used by this call only.
  * ---------------------------------------------------------------------------------- */
@@ -851,7 +852,8 @@ int hpmn_gated_scan_bwd(const HpmnGatedScanBwd *args, void *stream);
  *           A row whose index is outside [0, n_users) leaves the store alone and gets y = NaN.
  *   HPMN_STEP_COMMIT: the new state is written to the store.  Rows that name the same user are then applied in row order
  *           (each sees the state the one before it left); at most HPMN_STEP_MAX_INDEXED rows with `user` in that form.
- *   without it: the store is read only -- a candidate event scored "as if it were the next one"; rows are independent. */
+ *   without it: the store is read only -- a candidate event scored "as if it were the next one"; rows are independent.
+ *   y may be z or v itself; otherwise no output (y, a committed state) overlaps an input or the other (HPMN_EINVAL). */
 #define HPMN_STEP_COMMIT 1
 #define HPMN_STEP_USER_I64 2
 #define HPMN_STEP_MAX_INDEXED 4096

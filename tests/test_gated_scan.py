@@ -573,3 +573,82 @@ def test_step_on_infinite_states():
         state = torch.full((1, 5), bad, device="cuda")
         y = ops.gated_scan_step(z, v, state)
         assert (y == bad).all() and (state == bad).all()
+
+
+# ---------------------------------------------------------------------------------------------------------- overlapping memory
+def _apart(cls):
+    """Descriptors whose operands all lie apart, 1 MiB each."""
+    a = cls()
+    a.B, a.C, a.dtype = 2, 16, _lib.HPMN_BF16
+    for i, f in enumerate(f for f, t in cls._fields_ if t is C.c_void_p):
+        setattr(a, f, (i + 1) << 20)
+    for f, t in cls._fields_:
+        if f.endswith("_st") or f in ("z_s", "v_s", "y_s"):
+            setattr(a, f, 16)
+        elif f.endswith("_sb"):
+            setattr(a, f, 16 * 8 if f != "h0_sb" else 16)
+    return a
+
+
+@pytest.mark.parametrize("field,at", [("y", "z"), ("y", "v"), ("h_last", "h0"), ("saved", "z"), ("y", "begin"), ("y", "h_last"), ("saved", "y")])
+def test_forward_outputs_have_memory_of_their_own(lib, field, at):
+    a = _apart(_lib.HpmnGatedScan)
+    a.T, a.period = 8, 1
+    setattr(a, field, getattr(a, at))
+    assert lib.hpmn_gated_scan_fwd(C.byref(a), None) == -1
+
+
+@pytest.mark.parametrize("field,at,by", [("d_z", "z", 0), ("d_z", "v", 0), ("d_v", "z", 16), ("d_v", "d_y", 0), ("d_z", "saved", 64), ("d_v", "d_h_last", 0),
+                                         ("d_z", "d_v", 0), ("d_z", "d_v", 16), ("d_v", "d_z", 2 * (2 * 8 * 16) - 2), ("d_h0", "d_h_last", 0), ("d_v", "begin", 0)])
+def test_gradients_have_memory_of_their_own(lib, field, at, by):
+    a = _apart(_lib.HpmnGatedScanBwd)
+    a.T, a.period = 8, 1
+    setattr(a, field, getattr(a, at) + by)
+    assert lib.hpmn_gated_scan_bwd(C.byref(a), None) == -1
+
+
+@pytest.mark.parametrize("flags", [_lib.HPMN_STEP_COMMIT, 0])
+@pytest.mark.parametrize("field,at,by", [("y", "state", 0), ("y", "user", 0), ("y", "z", 2), ("v", "state", 64), ("z", "state", 0), ("user", "state", 4)])
+def test_a_store_has_memory_of_its_own(lib, field, at, by, flags):
+    a = _apart(_lib.HpmnGatedStep)
+    a.flags, a.n_users, a.state_s = flags, 9, 16
+    if not flags and field in ("z", "v", "user"):
+        pytest.skip("a store that is only read may be read twice")
+    setattr(a, field, getattr(a, at) + by)
+    assert lib.hpmn_gated_scan_step(C.byref(a), None) == -1
+
+
+@pytest.mark.gpu
+def test_wrappers_refuse_overlapping_buffers():
+    B, T, Cc = 2, 300, 12
+    z, v = inputs(B, T, Cc, torch.float32)
+    d_y = torch.randn(B, T, Cc, device="cuda")
+    _, _, saved = ops.gated_scan_fwd(z, v, train=True)
+    want = ops.gated_scan_bwd(z, v, saved, d_y)
+    wide = torch.empty(B, T, 3 * Cc, device="cuda")
+    long = torch.empty(B, 2 * T, Cc, device="cuda")
+    new = lambda: torch.empty_like(z)  # noqa: E731
+    for out in ((z, v), (new(), d_y), (d_y, new()), (z, new()), (wide[..., :Cc], wide[..., 1:Cc + 1]), (wide[..., :Cc], wide[..., Cc - 1:2 * Cc - 1]),
+                (long[:, :T], long[:, 1:T + 1]), (long[:, :T], long[:, T - 1:-1]), (new(), saved.new_empty(0))):
+        with pytest.raises(ValueError):
+            ops.gated_scan_bwd(z, v, saved, d_y, out=out)
+    # different columns of common rows, the first and the last steps of one buffer, other sequences of it
+    both = torch.empty(2 * B, T, Cc, device="cuda")
+    for out in ((wide[..., :Cc], wide[..., Cc:2 * Cc]), (wide[..., 2 * Cc:], wide[..., 1:Cc + 1]), (long[:, :T], long[:, T:]), (long[:, T:], long[:, :T]),
+                (both[:B], both[B:]), (both[0::2], both[1::2])):
+        got = ops.gated_scan_bwd(z, v, saved, d_y, out=out)
+        assert all(torch.equal(g, w) for g, w in zip(got, want)) and got[0] is out[0] and got[1] is out[1]
+    # inputs and gradients side by side in one buffer
+    row = torch.empty(B, T, 5 * Cc, device="cuda")
+    for i, t in enumerate((z, v, d_y)):
+        row[..., i * Cc:(i + 1) * Cc] = t
+    z2, v2, d2, o1, o2 = (row[..., i * Cc:(i + 1) * Cc] for i in range(5))
+    assert all(torch.equal(g, w) for g, w in zip(ops.gated_scan_bwd(z2, v2, saved, d2, out=(o1, o2)), want))
+    store, user = torch.randn(9, 2 * Cc, device="cuda"), torch.tensor([3, 4], device="cuda")
+    for call in (lambda: ops.gated_scan_step(store[:2, :Cc], z[:, 0], store[:, :Cc], user), lambda: ops.gated_scan_step(z[:, 0], store[5:7, 1:Cc + 1], store[:, :Cc], user)):
+        with pytest.raises(ValueError):
+            call()
+    before = store.clone()
+    y = ops.gated_scan_step(z[:, 0], store[:2, Cc:], store[:, :Cc], user)              # the other half of the store's rows
+    assert torch.equal(y, ops.gated_scan_step(z[:, 0], before[:2, Cc:].clone(), before[:, :Cc].clone(), user))
+    ops.gated_scan_step(store[:2, :Cc], z[:, 0], store[:, :Cc], user, commit=False)    # only read
