@@ -179,6 +179,10 @@ int hpmn_dropout(const HpmnDropout *a, void *stream) {
     if (!is_aligned(a->rng, 8)) return HPMN_EINVAL;
     if (a->x_s < 0 || a->r_s < 0 || (a->N > 1 && a->y_s < a->C)) return HPMN_EINVAL;
     if (a->N > ((1l << 34) - 1024) / a->C) return HPMN_EUNSUPPORTED;     // a launch: below 2^32 threads, four elements or more each
+    const int64_t es = elem_size(a->dtype);
+    const Region y = rows_of(a->y, a->N, a->y_s, a->C, es), x = rows_of(a->x, a->N, a->x_s, a->C, es), r = rows_of(a->residual, a->N, a->r_s, a->C, es);
+    const auto itself = [&](const void *p, int64_t stride) { return p == a->y && (a->N == 1 || stride == a->y_s); };
+    if ((!itself(a->x, a->x_s) && !apart(y, x)) || (!itself(a->residual, a->r_s) && !apart(y, r)) || !apart(y, Region(a->rng, 16))) return HPMN_EINVAL;
     // floor(p 2^16 + 1/2), as a double: p is a float, so the product is exact
     const double q = (double)a->keep_prob * 65536.0 + 0.5;
     const unsigned thr = q < 1.0 ? 1u : (unsigned)q;

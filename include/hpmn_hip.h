@@ -881,8 +881,8 @@ int hpmn_gated_scan_step(const HpmnGatedStep *args, void *stream);
  *   [offset, offset + ceil(N C / 4)); seeds are mixed, so neighbouring seeds have unrelated streams.
  *   rng    : optional 2 device uint64 {seed, offset}: used as seed = rng[0], offset += rng[1] (read by the kernel: a
  *            captured graph draws anew when the caller advances them between replays).
- *   x, residual (optional), y: [N, C] of dtype, row strides x_s / r_s / y_s in elements, dense columns.  y == x and
- *            y == residual are fine.  fp32 arithmetic, rounded once.
+ *   x, residual (optional), y: [N, C] of dtype, row strides x_s / r_s / y_s in elements, dense columns.  y may be x
+ *            or residual itself (same pointer and stride), any other overlap is HPMN_EINVAL.  fp32 arithmetic, rounded once.
  * ---------------------------------------------------------------------------------- */
 typedef struct HpmnDropout {
     int64_t N, C;

@@ -220,3 +220,32 @@ def test_more_than_32_bits_of_elements():
     for row in (0, 1 << 15, N - 1):
         m = oracle_mask(C_, 0.5, 4, row * C_ // 4)
         assert (y[row].double().cpu().numpy() == m).all()
+
+
+@pytest.mark.parametrize("x,x_s,r,r_s,y,y_s,rng", [(4096, 8, None, 0, 4096, 16, None), (4096, 16, None, 0, 4096, 8, None), (4096, 8, None, 0, 4098, 8, None),
+                                                   (4096, 0, None, 0, 4096, 8, None), (4096, 8, 8192, 16, 8192, 8, None), (4096, 8, 8192, 8, 8192 + 46, 8, None),
+                                                   (4096, 8, None, 0, 8192, 8, 8192 + 24)])
+def test_in_place_is_the_same_rows_or_refused(lib, x, x_s, r, r_s, y, y_s, rng):
+    """A row that a thread writes must be no row that another one has yet to read."""
+    a = _args()
+    a.x, a.x_s, a.residual, a.r_s, a.y, a.y_s, a.rng = x, x_s, r, r_s, y, y_s, rng
+    assert lib.hpmn_dropout(C.byref(a), None) == -1
+
+
+@pytest.mark.gpu
+def test_in_place_over_strided_rows_and_beside_other_columns(lib):
+    for cols in (slice(0, 48), slice(48, 96)):
+        buf = torch.randn(100, 96, device="cuda")
+        other = buf[:, :48] if cols.start else buf[:, 48:]
+        x, kept = buf[:, cols], other.clone()
+        want, beside = ops.dropout_fwd(x, 0.5, 77), ops.dropout_fwd(x, 0.5, 78)
+        a = _lib.HpmnDropout()
+        a.N, a.C, a.dtype, a.keep_prob, a.x_s, a.y_s = 100, 48, _lib.HPMN_F32, 0.5, 96, 96
+        a.x = x.data_ptr()
+        for seed, y in ((78, other), (77, x)):
+            a.seed, a.y = seed, y.data_ptr()
+            _lib.check(lib.hpmn_dropout(C.byref(a), torch.cuda.current_stream().cuda_stream), "hpmn_dropout")
+            if seed == 78:
+                assert torch.equal(other, beside)
+                other.copy_(kept)
+        assert torch.equal(x, want) and torch.equal(other, kept)
