@@ -1818,6 +1818,10 @@ def dropout_bwd(d_y, keep_prob, seed, *, offset=0, rng=None):
     return _dropout("dropout_bwd", d_y, keep_prob, seed, offset, None, rng)
 
 
+# Most bytes of scratch of one call (two parts in fp32 of every row and head come to 4 GiB at 4 M rows of 128); larger batches are cut up.
+_ATTN_WORKSPACE_MOST = 1 << 32
+
+
 def shared_prefix_attention(q, k_prefix, v_prefix, k_suffix=None, v_suffix=None, *, prefix_len=None, suffix_len=None, scale=None,
                             want_lse=False):
     """hpmn_prefix_attn: softmax attention of a batch whose rows share a long prefix (many candidates against one history; the
@@ -1866,8 +1870,25 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k_suffix=None, v_suffix=None,
                                 _ptr(suffix_len), out.data_ptr(), Lq * Hq * D, Hq * D, D, _ptr(lse), None, 0)
         lib = _lib.load()
         a.workspace_bytes = lib.hpmn_prefix_attn_workspace_bytes(C.byref(a))
+        while a.workspace_bytes > _ATTN_WORKSPACE_MOST and a.B > 1:
+            a.B = (a.B + 1) // 2
+            a.workspace_bytes = lib.hpmn_prefix_attn_workspace_bytes(C.byref(a))
         # per call: the caching allocator keeps it on the call's stream, and a captured graph owns its own
         ws = torch.empty(a.workspace_bytes, device=dev, dtype=torch.uint8) if a.workspace_bytes else None
         a.workspace = _ptr(ws)
         _call_on(dev, "hpmn_prefix_attn", lib.hpmn_prefix_attn, a)
+        for lo in range(a.B, B, a.B):                    # a batch cut up for its workspace: the rest of it, one piece behind the other
+            rest, a.B = slice(lo, min(lo + a.B, B)), min(a.B, B - lo)
+            if lib.hpmn_prefix_attn_workspace_bytes(C.byref(a)) > a.workspace_bytes:   # (a smaller last piece may be cut finer along the keys)
+                a.workspace_bytes = lib.hpmn_prefix_attn_workspace_bytes(C.byref(a))
+                ws = torch.empty(a.workspace_bytes, device=dev, dtype=torch.uint8)
+                a.workspace = _ptr(ws)
+            a.q, a.out = q[rest].data_ptr(), out[rest].data_ptr()
+            if S:
+                a.k_suf, a.v_suf = k_suffix[rest].data_ptr(), v_suffix[rest].data_ptr()
+            if suffix_len is not None:
+                a.suffix_len = suffix_len[rest].data_ptr()
+            if want_lse:
+                a.lse = lse[rest].data_ptr()
+            _call_on(dev, "hpmn_prefix_attn", lib.hpmn_prefix_attn, a)
     return (out, lse) if want_lse else out

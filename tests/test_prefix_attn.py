@@ -479,3 +479,29 @@ def test_refusals_are_value_errors():
         with pytest.raises(ValueError):
             call()
             pytest.fail("call %d was accepted" % i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(37, 1, 4, 2, 64, 900, 30), (5, 9, 4, 2, 40, 300, 30), (600, 1, 2, 1, 64, 400, 3), (64, 1, 2, 1, 32, 500, 0)])
+def test_large_batches_are_cut_up_for_their_workspace(size, monkeypatch):
+    """With as little scratch as one sequence needs, and some amounts above: the same results, to the tolerances of check()."""
+    B, Lq, Hq, Hkv, D, P, S = size
+    x = inputs(*size, torch.bfloat16, seed=sum(size))
+    slen = torch.randint(0, S + 1, (B,), generator=torch.Generator().manual_seed(3), dtype=torch.int32).cuda() if S else None
+    made, empty = [], torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: made.append(empty(*a, **k)) or made[-1])
+    check(*x, slen=slen)
+    whole = max((t.numel() for t in made if t.dtype == torch.uint8), default=0)
+    assert (whole > 0) == (size[-1] > 0)                               # (the short prefix by itself needs none: nothing to cut)
+    for most in (0, whole // 5, whole // 2 + 1):
+        made.clear()
+        monkeypatch.setattr(ops, "_ATTN_WORKSPACE_MOST", most)
+        check(*x, slen=slen)
+        assert max((t.numel() for t in made if t.dtype == torch.uint8), default=-1) < whole
+
+
+def test_the_largest_batches_need_more_scratch_than_one_call_takes(lib):
+    """What is cut up: 2^25 rows and 2^26 rows of 128 with keys of their own ask for tens of GB."""
+    a = _args()
+    a.B, a.Lq, a.Hq, a.Hkv, a.D, a.P, a.S = 1 << 19, 4, 16, 4, 128, 512, 48
+    assert lib.hpmn_prefix_attn_workspace_bytes(C.byref(a)) > 8 * ops._ATTN_WORKSPACE_MOST
