@@ -90,8 +90,10 @@ __device__ __forceinline__ T *at_row(T *p, unsigned row, int64_t stride) {
 
 // A lane's share of the work: its channels [c, c + n) (n = 0: none, it repeats another lane's loads and stores nothing), and the
 // steps [lo, hi) that count.  Where C is no multiple of four the last quad ends at C and computes some of the channels of the one in front
-// of it again, to the same values: whole quads at any alignment beat scalar accesses (500 x 1024 x 63 fp32,
-// forward / backward 61 / 124 us against 95 / 210; 7 x 3592 x 234 fp16 22 / 30 against 34 / 53).  Loads always go to a row in [lo, hi) (to one valid row if there is none), so that none is conditional.
+// of it again, to the same values: whole quads at any alignment beat scalar accesses (500 x 1024 x 63 fp32 forward + backward 184 us
+// against 305 when it was measured; now 80 / 133 against 80 / 137 for 64 channels.  A bf16 row of 1023 straddles cache lines: 16 x 4096 x
+// 1023 125 / 213 against 85 / 150 for 1024).  Loads always go to a row in [lo, hi) (to one valid row if there is none), so that none is
+// conditional.
 struct Share {
     int c, n, nl, lo, hi;
     __device__ __forceinline__ Share(int C, int T, int first, int begin) {
@@ -148,8 +150,8 @@ struct ChunkArgs {
     int chunks, tiles;                       // per sequence, per chunk
 };
 
-// Bound by memory latency more than rate (a lane group walks its span alone, loads four steps ahead): 1 x 65536 x 256 bf16 14.8 us
-// for 67 MB, 4.5 TB/s; behind it the main kernel finds z and v in the cache, 24.2 us.
+// Bound by memory latency more than rate (a lane group walks its span alone, loads four steps ahead): 1 x 65536 x 256 bf16 14.3 us
+// for 67 MB, 4.7 TB/s; behind it the main kernel finds z and v in the cache, 26.9 us.
 template <typename T, int LPR, bool VEC, bool BWD>
 __global__ __launch_bounds__(512) void gated_scan_chunk_kernel(const ChunkArgs a) {
     constexpr int TG = 64 / LPR;
@@ -280,8 +282,9 @@ __device__ __forceinline__ v4f fold_chunks(const float *ws, int C, int c, int nl
     return start;
 }
 
-// Memory-bound: 500 x 1024 x 64 fp32, period 2, 328 MB in 71.6 us, 4.6 TB/s (a copy reaches 4.7); 16 x 4096 x 1024 bf16, 403 MB in
-// 81.4 us, 4.9 TB/s.  Small calls are a launch and one round trip to memory: 128 x 100 x 32 fp32 4.9 us.
+// Memory-bound: 500 x 1024 x 64 fp32, period 2, 328 MB in 72.2 us, 4.5 TB/s, the waves waiting 41 % of their cycles (a copy reaches
+// 4.7, the backward below 5.5: not the memory's limit, but what loads one tile ahead ask of it).  16 x 4096 x 1024 bf16, 403 MB in
+// 84.8 us, 4.8 TB/s.  Small calls are a launch and one round trip to memory: 128 x 100 x 32 fp32 5.1 us.
 template <typename T, int LPR, bool VEC>
 __global__ __launch_bounds__(512) void gated_scan_fwd_kernel(const HpmnGatedScan a, int chunks, int chunk_tiles) {
     constexpr int TG = 64 / LPR;             // runs side by side in a wave
@@ -365,8 +368,9 @@ __global__ __launch_bounds__(512) void gated_scan_fwd_kernel(const HpmnGatedScan
     if (a.h_last && chunk == chunks - 1 && threadIdx.x < LPR) store_state(a.h_last + b * a.C + sh.c, carry, sh.n);
 }
 
-// Memory-bound: 500 x 1024 x 64 fp32, period 2, 590 MB in 105.9 us, 5.6 TB/s; 16 x 4096 x 1024 bf16, 671 MB in 149 us, 4.5 TB/s
-// (256 workgroups there, one a CU, whose waves wait for memory half of their cycles); 128 x 100 x 32 fp32 6.6 us.
+// Memory-bound: 500 x 1024 x 64 fp32, period 2, 590 MB in 106.8 us, 5.5 TB/s, behind its forward, which leaves some of z and v in the cache
+// (by itself, on inputs that are in no cache, 124 us); 16 x 4096 x 1024 bf16, 671 MB in 149.8 us, 4.5 TB/s (256 workgroups there, one
+// a CU, whose waves wait for memory half of their cycles); 128 x 100 x 32 fp32 7.0 us.
 template <typename T, int LPR, bool VEC>
 __global__ __launch_bounds__(512) void gated_scan_bwd_kernel(const HpmnGatedScanBwd a, int chunks, int chunk_tiles) {
     constexpr int TG = 64 / LPR;
@@ -585,14 +589,13 @@ struct Cut {
     int chunks, tiles;                       // per sequence, per chunk
 };
 // Time chunks where whole sequences leave two thirds of the CUs idle and there are at least four tiles to share out: as many as
-// fill the CUs once (twice costs more than it hides: the backward has the registers for one workgroup per CU), at most TILE of
-// them (fold_chunks).  Forward / backward us, cut against whole, fp32, C = 64, device time:
-//   8 x 1024: 11 / 14 against 19 / 28;   64 x 4096: 55 / 80 against 65 / 130;   1 x 16384: 14 / 17 against 241 / 379;
-//   at the rule's borders: 64 x 512 12.4 / 17.1 against 11.7 / 17.6, 80 x 1024 19 / 27 against 20 / 31;
-//   beyond them: 96 x 1024 (two chunks) 26 / 33 against 21 / 32, 8 x 256 (two tiles) 10 / 12 against 7 / 10.
-// Up to 32 (16) channels a workgroup has half (a quarter) of the waves, so the CUs are full with twice (four times) as many:
-//   49 x 7701 x 10 bf16 20 / 28 against 35 / 48 with 256, 64 x 4096 x 16 fp32 20 / 27 against 27 / 32, 84 x 1024 x 32 15.4 / 20.9 against
-//   15.2 / 20.0.
+// fill the CUs once (twice costs more than it hides: the backward has the registers, 202 to 231, for one workgroup per CU), at most
+// TILE of them (fold_chunks).  Forward / backward us, cut against whole, fp32, C = 64, device time:
+//   8 x 1024: 12 / 15 against 20 / 29;   64 x 4096: 58 / 87 against 79 / 133;   1 x 16384: 15 / 19 against 268 / 406;
+//   at the rule's borders: 64 x 512 14.3 / 18.1 against 12.5 / 18.3, 80 x 1024 20 / 30 against 21 / 35;
+//   beyond them: 96 x 1024 (two chunks) 28 / 37 against 21 / 38, 8 x 256 (two tiles) 10 / 13 against 7 / 10.
+// Up to 32 (16) channels a workgroup has half (a quarter) of the waves, so the CUs are full with twice (four times) as many: 49 x 7701 x
+// 10 bf16 20 / 28 against 35 / 48 with 256, 64 x 4096 x 16 fp32 20 / 27 against 27 / 32 when that was measured (24 / 32, 20 / 28 now).
 static Cut scan_cut(int B, int T, int C) {
     const int lpr = scan_lanes(C), tiles = (T + TILE - 1) / TILE;
     const long whole = (long)B * ((C + 4 * lpr - 1) / (4 * lpr));

@@ -15,13 +15,19 @@
 // A row's own suffix is the same thing with M = Lq Hq / Hkv rows and a key limit per row, in the same launch; a few keys of very many
 // sequences are left to the joining kernel.
 //
-// Bound by the matrix pipe for many rows: 512 x 16 heads over 4 of 128, 32768 keys + 64 own bf16, 137.6 GF: 160 us + 9.7 us of joining,
-// 0.86 PF/s in the first kernel (a library product of 8192^3 1.22; what is missing: the probabilities' share of issue slots, and the
-// own keys, 67 MB, behind the prefix).  fp32 (products of 32 x 32 x 2, 137 TF/s at most): 158 x 16 heads over 8 of 96, 7850 keys 115 us,
-// 66 TF/s.  Bound by launches and round trips for few: 8 rows of 64 over 1000 keys fp32 7.4 + 3.6 us.
+// Bound by the matrix pipe and the VALU together for many rows: 512 x 16 heads over 4 of 128, 32768 keys + 64 own bf16, 137.6 GF:
+// 160-168 us + 10 us of joining, 0.82-0.86 PF/s in the first kernel (a library product of 8192^3 1.22).  The matrix pipe is busy in
+// 44 % of the cycles, 6.6 other VALU instructions to an MFMA take about as many, and few of the two meet: the alternation gains
+// little over the sum.  fp16 the same: 16384 keys 93 us.  fp32 (products of 32 x 32 x 2, 137 TF/s at most): 512 x 16 heads over 4 of
+// 128, 8192 keys 353 us, 97 TF/s, the matrix pipe busy in 67 % of the cycles, the rest the exponentials and what the one wave a SIMD
+// that 348 registers allow cannot hide; 158 x 16 heads over 8 of 96, 7850 keys 108 us, 71 TF/s, 51 %: its 316 rows a key head fill 384.
+// Several query tokens: 512 x 48 tokens x 16 heads of 128 over 512 + 48 keys 301 us + 184 of joining, bound by the parts, 409 MB written
+// and read.  Bound by launches and round trips for few: 8 rows of 64 over 1000 keys fp32 7.4 + 3.6 us.
 //
 // Rounding choices: scores, maxima, sums and outputs are fp32; the probabilities are rounded to the 16-bit type once, as operand of
-// the second product (half a step each, independent, so about one more rounding of the result).  fp16 probabilities are scaled by
+// the second product: half a step of each, so at most half a step of sum p |v| beside the output's own rounding (reached where many
+// equal scores are rounded the same way), and about as much as that rounding where they differ.  The sum that divides stays unrounded,
+// so that lse is.  A second operand plane for what is rounded off would be half as many products again.  fp16 probabilities are scaled by
 // 2^12 (2^15 at most where the maximum lags): unscaled, everything below 2^-24 of the largest would vanish, which for long prefixes
 // is most of them; scaled, what is below 2^-26 of it starts to lose digits and 2^-36 vanishes.
 #pragma once

@@ -44,8 +44,8 @@ __device__ __forceinline__ void store_quad(T *p, v4f x, int n) {
     }
 }
 
-// a = sigmoid(z) = 1 / (1 + e) and u = 1 - a = e / (1 + e) with e = exp(-z): both to a rounding or two of THEMSELVES (1 - a as a
-// difference has no digits left from z = 17 on).  e is capped at 2^120, where a has long stopped mattering beside u = 1 (and
+// a = sigmoid(z) = 1 / (1 + e) and u = 1 - a = e / (1 + e) with e = exp(-z), each relative to ITSELF (1 - a as a difference has no digits
+// left from z = 17 on): a few roundings and the exponent's, about |z| 2^-24, in whichever of the two is small.  e is capped at 2^120, where a has long stopped mattering beside u = 1 (and
 // inf * 0 would be NaN); the cap is the minimum that keeps a NaN.  Six instructions, two of them on the transcendental unit.
 __device__ __forceinline__ void gate_pair(float z, float &a, float &u) {
     const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(NEG_LOG2E * z, 120.0f));

@@ -1572,7 +1572,9 @@ def read_fwd_bwd_n(descs, params, d_params, memories, lasts, label, masks, keep_
 
 
 # ---------------------------------------------------------------------------------------
-# sequence operators: the gated linear recurrence (time-parallel counterpart of the GRU scans above)
+# sequence operators: the gated linear recurrence (time-parallel counterpart of the GRU scans above), dropout, attention over a
+# shared prefix.  As everywhere in this module there is no autograd: a forward and its backward are two calls, an input that requires a
+# gradient is taken as data, and the results carry none.
 # ---------------------------------------------------------------------------------------
 _SEQ_DTYPES = {torch.float32: _lib.HPMN_F32, torch.bfloat16: _lib.HPMN_BF16, torch.float16: _lib.HPMN_F16}
 
@@ -1831,7 +1833,11 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k_suffix=None, v_suffix=None,
 
     ``prefix_len``: int32 [1] on the device, the prefix in use (None: P).  ``suffix_len``: int32 [B] (None: S); with several query
     tokens they are the last of the suffix and see it up to their own position.  ``scale``: default D ** -0.5.  Returns out
-    [B, Lq, Hq, D] (a query without any key: zeros), with ``want_lse`` also the log-sum-exp [B, Lq, Hq] float32 (-inf there)."""
+    [B, Lq, Hq, D] (a query without any key: zeros), with ``want_lse`` also the log-sum-exp [B, Lq, Hq] float32 (-inf there).
+
+    Forward only: for scoring, no backward exists.  Scores, softmax sums and the output are accumulated in float32; for 16-bit types the
+    probabilities are rounded to the type before they multiply the values, at most half a step of the weighted average of |v| beside
+    out's own rounding (lse is not touched by that)."""
     dt, dev = _seq_input("q", q, 4), q.device
     B, Lq, Hq, D = q.shape
     if k_prefix.dim() != 3:

@@ -908,7 +908,9 @@ int hpmn_dropout(const HpmnDropout *args, void *stream);
  *   suffix_len : optional [B] device int32, clamped to [0, S]; NULL: S.  The Lq query tokens are the suffix's last: token i sees
  *                suffix keys j < suffix_len - Lq + 1 + i (one query token: all of them) and the whole prefix.
  * Keys and values behind the lengths are not looked at.  A query that sees no key at all gets out = 0, lse = -inf.
- * D <= 128.  Scores, maxima, sums and the output accumulator are fp32 for every dtype.
+ * D <= 128.  Scores, maxima, sums and the output accumulator are fp32 for every dtype; for bf16 and fp16 the probabilities are rounded to
+ * the dtype before they multiply the values (the sum that divides is not), so beside out's own rounding it is off by at most half a step
+ * of the average of |v| under the weights.  Forward only.
  * workspace: >= hpmn_prefix_attn_workspace_bytes(args) bytes (16-byte aligned; the size depends on the sizes alone).
  * ---------------------------------------------------------------------------------- */
 typedef struct HpmnPrefixAttn {
