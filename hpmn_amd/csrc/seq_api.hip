@@ -163,8 +163,8 @@ int hpmn_gated_scan_step(const HpmnGatedStep *a, void *stream) {
     const int64_t B = a->B, C = a->C, es = elem_size(a->dtype);
     const Region z = rows_of(a->z, B, a->z_s, C, es), v = rows_of(a->v, B, a->v_s, C, es), y = rows_of(a->y, B, a->y_s, C, es);
     const Region state = rows_of(a->state, a->n_users, a->state_s, C, 4), user(a->user, B * (a->flags & HPMN_STEP_USER_I64 ? 8 : 4));
-    if (!apart(y, state) || !apart(y, user) || (!(a->y == a->z && a->y_s == a->z_s) && !apart(y, z)) || (!(a->y == a->v && a->y_s == a->v_s) && !apart(y, v)))
-        return HPMN_EINVAL;
+    const auto itself = [&](const void *p, int64_t stride) { return p == a->y && (B == 1 || stride == a->y_s); };
+    if (!apart(y, state) || !apart(y, user) || (!itself(a->z, a->z_s) && !apart(y, z)) || (!itself(a->v, a->v_s) && !apart(y, v))) return HPMN_EINVAL;
     if ((a->flags & HPMN_STEP_COMMIT) && !(apart(state, z) && apart(state, v) && apart(state, user))) return HPMN_EINVAL;
     return gated_step_launch(*a, (hipStream_t)stream);
 }

@@ -1734,7 +1734,7 @@ def gated_scan_step(z, v, state, user=None, *, commit=True):
 
     ``commit``: the new states are written to the store; events of the same user are applied in row order.  Without it the store
     is only read (a candidate event scored as if it were the next one; any user may be named any number of times).  A row whose
-    user is outside the store changes nothing and gets NaN."""
+    user is outside the store changes nothing and gets NaN.  A store that is written shares no memory with z, v or user (refused)."""
     code, shape, dev = _seq_input("z", z, 2), z.shape, z.device
     B, Cc = shape
     _chk_seq("v", v, shape, z.dtype, dev)

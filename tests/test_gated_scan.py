@@ -652,3 +652,20 @@ def test_wrappers_refuse_overlapping_buffers():
     y = ops.gated_scan_step(z[:, 0], store[:2, Cc:], store[:, :Cc], user)              # the other half of the store's rows
     assert torch.equal(y, ops.gated_scan_step(z[:, 0], before[:2, Cc:].clone(), before[:, :Cc].clone(), user))
     ops.gated_scan_step(store[:2, :Cc], z[:, 0], store[:, :Cc], user, commit=False)    # only read
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,y_s", [(5, 40), (1, 24), (1, 40)])
+@pytest.mark.parametrize("over", ["z", "v"])
+def test_step_in_place_through_the_c_abi(lib, B, y_s, over):
+    """y over z's or v's own rows: the same stride, or a single row, whatever its stride is said to be."""
+    Cc = 24
+    x = {n: torch.randn(B, 40, generator=torch.Generator().manual_seed(i)).cuda() for i, n in enumerate("zv")}
+    state = torch.randn(B, Cc, device="cuda")
+    want_state = state.clone()
+    want = ops.gated_scan_step(x["z"][:, :Cc].clone(), x["v"][:, :Cc].clone(), want_state)
+    a = _lib.HpmnGatedStep()
+    a.B, a.C, a.dtype, a.flags, a.n_users, a.state_s, a.z_s, a.v_s, a.y_s = B, Cc, _lib.HPMN_F32, _lib.HPMN_STEP_COMMIT, B, Cc, 40, 40, y_s
+    a.z, a.v, a.y, a.state = x["z"].data_ptr(), x["v"].data_ptr(), x[over].data_ptr(), state.data_ptr()
+    _lib.check(lib.hpmn_gated_scan_step(C.byref(a), torch.cuda.current_stream().cuda_stream), "hpmn_gated_scan_step")
+    assert torch.equal(x[over][:, :Cc], want) and torch.equal(state, want_state)
